@@ -167,17 +167,12 @@ def work(case):
             "flops": 4 * pairs * case["heads"] * case["dim"]}
 
 
-def _power(e):
-    """2^e in 32 bits, exactly: the exponent field itself."""
-    return ((e.int() + 127) << 23).view(torch.float32)[..., None]
-
-
 def _quantise(x, dtype):
     """e4m3 codes and exponents of rows: the least power of two at which the row's largest value is at most 448."""
     x = x.float()
     mant, e = torch.frexp(x.abs().amax(-1))
     e = torch.where(mant == 0, torch.full_like(e, -126), torch.where(mant <= 0.875, e - 9, e - 8).clamp(-126, 120))
-    y = x * _power(-e)
+    y = torch.ldexp(x, -e[..., None])
     most = torch.where(e >= LARGEST[dtype], 240.0, 448.0)[..., None]
     return torch.minimum(torch.maximum(y, -most), most).to(torch.float8_e4m3fn), e.to(torch.int8)
 
@@ -289,7 +284,7 @@ def _plain_write(s):
 
 def _values(s, name):
     pages = s[name + "_pages"].float()
-    return pages if s[name + "_exp"] is None else pages * _power(s[name + "_exp"])
+    return pages if s[name + "_exp"] is None else torch.ldexp(pages, s[name + "_exp"][..., None].int())
 
 
 def _plain_read(s):
@@ -413,21 +408,17 @@ def _exact_norm_rope(case, s):
     return got
 
 
-def _two_to(e):
-    return ((e.long() + 1023) << 52).view(torch.float64)
-
-
 def _exact_codes(x, dtype):
     x = x.double()
     largest = x.abs().amax(-1, keepdim=True)
     e = torch.full_like(largest, -126.0)
     some = largest > 0
     e[some] = torch.ceil(torch.log2(largest[some] / 448)).clamp(-126, 120)
-    e = torch.where(largest > 448 * _two_to(e), e + 1, e)
-    e = torch.where((largest <= 448 * _two_to(e - 1)) & (e > -126) & some, e - 1, e)
-    y = x / _two_to(e)
+    e = torch.where(largest > 448 * 2.0 ** e, e + 1, e)
+    e = torch.where((largest <= 448 * 2.0 ** (e - 1)) & (e > -126) & some, e - 1, e)
+    y = x / 2.0 ** e
     most = torch.where(e >= LARGEST[dtype], 240.0, 448.0)
-    step = _two_to(torch.frexp(y.abs().clamp_min(2.0 ** -6))[1] - 4)
+    step = 2.0 ** (torch.floor(torch.log2(y.abs().clamp_min(2.0 ** -6))) - 3)
     return torch.minimum(torch.maximum(torch.round(y / step) * step, -most), most), e[..., 0]
 
 
@@ -460,7 +451,7 @@ def _context(case, s, name, b, kv):
     pages = s["table"][b, :n].long()
     rows = s[name + "_pages"][pages].double()
     if s[name + "_exp"] is not None:
-        rows = rows * _two_to(s[name + "_exp"][pages])[..., None]
+        rows = rows * 2.0 ** s[name + "_exp"][pages].double()[..., None]
     return rows.transpose(0, 1).reshape(case["kv_heads"], n * case["page"], case["dim"])[:, :kv]
 
 
