@@ -1048,12 +1048,19 @@ int magb200_matmul_swiglu(int device, const magb200_view_t *x, const magb200_vie
 }
 
 // ---- head norm + rotation, paged KV cache, attention -----------------------------------------------------------------------
+// Kernels load whole elements: an address between two of them would end the context.
+static int on_elements(const void *p, size_t bytes, const char *what) {
+    if ((uintptr_t)p % bytes == 0) return MAGB200_OK;
+    set_error("%s: address %p is not a multiple of the element size %zu", what, p, bytes);
+    return MAGB200_ERR_INVALID_ARG;
+}
 static int head_rows(const magb200_view_t *v, const char *what, HeadRows *r) {
     if (int rc = check_view(v, what)) return rc;
     if (v->rank != 3) { set_error("%s: [tokens][heads][head_dim] expected, got rank %d", what, v->rank); return MAGB200_ERR_SHAPE; }
     if (v->shape[2] != 1 && v->strides[2] != 1) { set_error("%s: the elements of a head must be neighbours (stride %lld)", what, (long long)v->strides[2]); return MAGB200_ERR_INVALID_ARG; }
     if (v->shape[1] > 65535) { set_error("%s: %lld heads", what, (long long)v->shape[1]); return MAGB200_ERR_TOO_LARGE; }
     r->p = view_data(v);
+    if (int rc = on_elements(r->p, dtype_size(v->dtype), what)) return rc;
     r->token_stride = v->strides[0];
     r->head_stride = v->strides[1];
     r->heads = (int)v->shape[1];
@@ -1130,6 +1137,8 @@ static int make_batch(const magb200_kv_batch_t *b, const char *what, int64_t tok
         set_error("%s: batch %d, max_pages %d, max_q %d, max_kv %d", what, b->batch, b->max_pages, b->max_q, b->max_kv);
         return MAGB200_ERR_INVALID_ARG;
     }
+    const void *arrays[3] = {b->kv_len, b->pages, needs_q ? b->cu_q : nullptr};
+    for (const void *p : arrays) if (int rc = on_elements(p, sizeof(int32_t), what)) return rc;
     if (tokens > INT32_MAX) { set_error("%s: %lld rows", what, (long long)tokens); return MAGB200_ERR_TOO_LARGE; }
     const int64_t room = (int64_t)b->max_pages * page_size;
     out->cu_q = b->cu_q; out->kv_len = b->kv_len; out->table = b->pages;
@@ -1172,6 +1181,7 @@ int magb200_qk_norm_rope(int device, const magb200_view_t *q, const magb200_view
         if ((rc = check_view(w[i], "qk_norm_rope weight"))) return rc;
         if (w[i]->rank != 1 || w[i]->shape[0] != dim) { set_error("qk_norm_rope: a weight has one element per element of a head"); return MAGB200_ERR_SHAPE; }
         if (w[i]->dtype != q->dtype || w[i]->strides[0] != 1) { set_error("qk_norm_rope: weights are contiguous and of q's dtype"); return MAGB200_ERR_INVALID_ARG; }
+        if ((rc = on_elements(view_data(w[i]), dtype_size(w[i]->dtype), "qk_norm_rope weight"))) return rc;
     }
     if ((q_weight || k_weight) && !(eps >= 0.0 && eps <= 1.0)) { set_error("qk_norm_rope: eps %g is outside [0, 1]", eps); return MAGB200_ERR_INVALID_ARG; }
     RopeArgs r;
@@ -1179,6 +1189,7 @@ int magb200_qk_norm_rope(int device, const magb200_view_t *q, const magb200_view
     if (rope) {
         if (rope->rotary_dim < 2 || rope->rotary_dim > dim || rope->rotary_dim % 2) { set_error("qk_norm_rope: %d of %lld elements cannot be turned in pairs", rope->rotary_dim, (long long)dim); return MAGB200_ERR_INVALID_ARG; }
         if (!rope->positions || !rope->inv_freq || !isfinite(rope->factor)) { set_error("qk_norm_rope: null positions or frequencies, or a factor that is not finite"); return MAGB200_ERR_INVALID_ARG; }
+        if ((rc = on_elements(rope->positions, sizeof(int32_t), "qk_norm_rope positions")) || (rc = on_elements(rope->inv_freq, sizeof(float), "qk_norm_rope frequencies"))) return rc;
         r.positions = rope->positions; r.inv_freq = rope->inv_freq; r.rotary = rope->rotary_dim; r.interleaved = rope->interleaved != 0; r.factor = rope->factor;
     }
     // a result is its own input or apart from everything else the call touches
@@ -1241,6 +1252,7 @@ int magb200_kv_cache_read(int device, const magb200_kv_cache_t *cache, const mag
     KvBatch b;
     HeadRows rk, rv;
     if (!cu_kv) { set_error("kv_cache_read: null cu_kv"); return MAGB200_ERR_INVALID_ARG; }
+    if ((rc = on_elements(cu_kv, sizeof(int32_t), "kv_cache_read cu_kv"))) return rc;
     if ((rc = make_cache(cache, "kv_cache_read", &c)) || (rc = cache_rows(c, k, v, "kv_cache_read", &rk, &rv)) ||
         (rc = make_batch(batch, "kv_cache_read", k->shape[0], c.page_size, false, &b))) return rc;
     if (!rows_apart(k) || !rows_apart(v) || !rows_disjoint(k, v)) { set_error("kv_cache_read: rows of the results overlap"); return MAGB200_ERR_INVALID_ARG; }
@@ -1278,6 +1290,7 @@ int magb200_paged_attention(int device, const magb200_view_t *q, const magb200_k
             set_error("paged_attention: lse is a contiguous float32 [tokens][heads]");
             return MAGB200_ERR_SHAPE;
         }
+        if ((rc = on_elements(view_data(lse), sizeof(float), "paged_attention lse"))) return rc;
         const AddrRange l = view_range(lse), x = view_range(q), o = view_range(out);
         if ((l.lo < x.hi && x.lo < l.hi) || (l.lo < o.hi && o.lo < l.hi)) { set_error("paged_attention: lse overlaps q or the result"); return MAGB200_ERR_INVALID_ARG; }
         if (in_pools(a.cache, l)) { set_error("paged_attention: lse lies in the cache"); return MAGB200_ERR_INVALID_ARG; }

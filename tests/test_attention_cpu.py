@@ -217,3 +217,27 @@ def test_the_oracles_codes():
     assert A.e4m3_codes(np.array([17.0, 19.0, 2.0 ** -10, 3 * 2.0 ** -10])).tolist() == [0x58, 0x5A, 0x00, 0x02]
     codes, exps = A.quantise(np.array([[448.0, 1.0], [449.0, 1.0], [0.0, 0.0], [np.inf, 1.0]]), O.BFLOAT16)
     assert exps.tolist() == [0, 1, -126, -128] and codes[0].tolist() == [0x7E, 0x38]
+
+
+def test_addresses_between_two_elements_are_refused():
+    """A load of an element that is not on a multiple of its size ends a device's context, so no such address gets there."""
+    rows, out, w = (6, 2, 64), tensor(Q, at=FAR), tensor((64,), at=16 * FAR)
+    odd, by_two = BASE + 1, BASE + 2
+
+    def refused_address(fn, *a, **kw):
+        assert "multiple of the element size" in refused(mb.ERR_INVALID_ARG, fn, *a, **kw)
+
+    for b in (dict(cu_q=by_two), dict(kv_len=odd), dict(pages=by_two)):
+        refused_address(mb.kv_cache_write, cache(), batch(**b), tensor(rows), tensor(rows))
+        refused_address(mb.paged_attention, tensor(Q), cache(), batch(**b), out)
+    refused_address(mb.kv_cache_write, cache(), batch(), tensor(rows, at=odd), tensor(rows))
+    refused_address(mb.kv_cache_write, cache(), batch(), tensor(rows), tensor(rows, at=odd))
+    refused_address(mb.kv_cache_read, cache(), batch(), by_two, tensor(rows), tensor(rows, at=FAR))
+    refused_address(mb.kv_cache_read, cache(), batch(), BASE, tensor(rows), tensor(rows, at=FAR + 1))
+    refused_address(mb.paged_attention, tensor(Q), cache(), batch(), out, lse=tensor((6, 4), mb.FLOAT32, at=2 * FAR + 2))
+    for at, dtype in ((odd, mb.BFLOAT16), (by_two, mb.FLOAT32)):
+        refused_address(mb.qk_norm_rope, tensor(Q, dtype, at=at), None, None, tensor(Q, dtype, at=FAR))
+        refused_address(mb.qk_norm_rope, tensor(Q, dtype), None, None, tensor(Q, dtype, at=FAR + at - BASE))
+        refused_address(mb.qk_norm_rope, tensor(Q, dtype), None, None, tensor(Q, dtype, at=FAR), q_weight=tensor((64,), dtype, at=16 * FAR + at - BASE))
+    for rope in (mb.Rope(by_two, BASE, 64), mb.Rope(BASE, by_two, 64)):
+        refused_address(mb.qk_norm_rope, tensor(Q), None, rope, out, q_weight=w)
