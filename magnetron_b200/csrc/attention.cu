@@ -219,8 +219,8 @@ __device__ __forceinline__ void attend_few(const AttentionArgs &a, int few_rows,
         }
 
         // ---- the rows' queries, in the registers for the whole kernel. Against codes the product is in fp16, which holds every code;
-        // bf16 queries are scaled by a power of two per row so that their largest element is in [1, 2): what falls below fp16's
-        // range then is under 2^-25 of it.
+        // bf16 queries are scaled by a power of two per row so that their largest element is in [1, 2), or in [2, 4) from 2^127 on, whose
+        // reciprocal is below the least normal number: what falls below fp16's range then is under 2^-25 of it.
         uint32_t qf[NT][kSteps][2];               // columns g8 of each group of 8 rows
         float row_factor[NT][2];                  // of rows 2c and 2c + 1: scale * log2(e), and back from that power of two
         int last[NT][2], first[NT][2];            // cached rows first .. last - 1 are seen by these rows
@@ -250,6 +250,7 @@ __device__ __forceinline__ void attend_few(const AttentionArgs &a, int few_rows,
                 top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
                 int e = (int)(top >> 7) - 127;
                 if (e < -126) e = -126;
+                if (e == 127) e = 126;
                 if (e == 128) e = 0;                                   // an infinity or a NaN stays one
                 factor = a.scale_log2 * pow2f(e);
                 const float inv = pow2f(-e);

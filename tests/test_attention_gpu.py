@@ -612,3 +612,28 @@ def test_a_layers_attention_block_prompt_then_tokens(gpu, bits):
         wf = O.bits_to_f64(dt, wo.to_bits())
         assert (np.abs(O.bits_to_f64(dt, y.to_bits()) - ob @ wf.T) <= (2.0 ** -8 + heads * dim * 2.0 ** -24) * (np.abs(ob) @ np.abs(wf).T)).all()
         done = kv_lens
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("q_lens", [[1], [2], [4], [40]])
+def test_query_rows_at_the_top_of_bf16(gpu, bits, q_lens):
+    """Rows whose largest element lies in [2^127, 2^128), against keys so small that their scores are ordinary numbers: of either
+    sign, beside rows of ordinary size, in tiles of 8, 16 and 32 rows and of 256."""
+    heads, n = 8, q_lens[0]
+    p = Paged(gpu, mb.BFLOAT16, bits, q_lens, [90], kv_heads=1, dim=64, page=16, seed=14)
+    rng = np.random.default_rng(14)
+    for page, slot in ((p.tables[0][i // 16], i % 16) for i in range(90)):
+        element, lift = int(rng.integers(8, 16)), int(rng.integers(0, 3))      # 1 .. 1.875 times 2^-124 .. 2^-122, and zeros beside it
+        if bits == 8:
+            p.pool["k"][page, 0, slot], p.exps["k"][page, 0, slot] = 0, -124 + lift
+            p.pool["k"][page, 0, slot, 5] = 0x30 + element                      # exponent field 7: 1.fff
+        else:
+            p.pool["k"][page, 0, slot] = 0
+            p.pool["k"][page, 0, slot, 5:6] = bits_of(mb.BFLOAT16, [element * 2.0 ** (-127 + lift)])
+    p.upload()
+    q = rng.standard_normal((n, heads, 64)).astype(np.float32)
+    q[:, 0, 5], q[:, 1, 5], q[:, 2, 5], q[:, 3, 5] = 2.0 ** 127, -1.9 * 2.0 ** 127, 2.0 ** 126, 1.5 * 2.0 ** 127
+    q[:, 3, 9] = -2.0 ** 127
+    qb = bits_of(mb.BFLOAT16, q)
+    got = mb.paged_attention(mb.Tensor.from_bits(gpu, mb.BFLOAT16, qb), p.cache, p.batch).to_bits()
+    check_attention(p, qb, got)
