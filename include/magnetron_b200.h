@@ -258,7 +258,9 @@ int  magb200_kv_cache_read(int device, const magb200_kv_cache_t *cache, const ma
  * last `window` of them (its own among them). Not causal: all kv_len[b] cached tokens, whatever the number of new ones (cross
  * attention). A row that sees nothing gives 0. lse (optional, f32 [tokens][heads], contiguous): the natural logarithm of the
  * sum of exponentials, -inf for a row that sees nothing. Scores, maxima, sums and the output's sums are fp32; the weights are
- * rounded to the dtype for their product with V. Results are the same from call to call. A cached row that the mask hides
+ * rounded to the dtype for their product with V (over 8-bit rows to f16 when the sequence has at most 32 (new token, query head)
+ * rows a KV head); f16 weights lose bits under 2^-21 of the row's
+ * largest, by 2^-32 of it at most. Results are the same from call to call. A cached row that the mask hides
  * from a row does not change it, except that a NaN or infinity in V does within a tile of up to 128 cached rows that the mask
  * crosses; rows of a page behind the last cached token are never used. */
 int  magb200_paged_attention(int device, const magb200_view_t *q, const magb200_kv_cache_t *cache, const magb200_kv_batch_t *batch,

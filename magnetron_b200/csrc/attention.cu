@@ -5,7 +5,7 @@
 // The query heads that share a KV head are rows of the same tiles: row r of a sequence is (new token r / group, query head
 // r % group), so that a cached row is read once for the whole group. One pass over the cached rows with the running maximum
 // and sum of the softmax (exp2 of scores scaled by log2 e), both in fp32, as are the output's sums; the weights are rounded
-// to the tensor type for their product with V. Long sequences are split along the cached rows over several CTAs, which leave
+// to 16 bits for their product with V: to the tensor type, or to fp16 for few rows over codes. Long sequences are split along the cached rows over several CTAs, which leave
 // (maximum, sum, output) of their part in the workspace, to be joined in the order of the parts.
 #include "attention_dev.cuh"
 
@@ -87,6 +87,10 @@ template <int DT, bool kEight, int DPAD, int NT>
 __device__ __forceinline__ void attend_few(const AttentionArgs &a, int few_rows, int least) {
     using Cfg = FewCfg<kEight, NT>;
     constexpr int MM = kEight ? (int)MAGB200_F16 : DT;             // type of the products
+    // fp16 weights are made 2^15 times as large, as far as the type reaches: they keep all their bits down to 2^-29 of the row's
+    // largest and are lost under 2^-40 of it, where many rows of small weight would otherwise go missing from the output (under
+    // 2^-25 unscaled: 0.2 % of 50000 rows) while the sum in fp32 counts them
+    constexpr float kLift = MM == MAGB200_F16 ? 15.0f : 0.0f;
     constexpr int kSteps = DPAD / 16, kPitch = Cfg::pitch(DPAD), kStage = Cfg::stage_bytes(DPAD), kRows = 8 * NT;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ int is_last;
@@ -282,9 +286,9 @@ __device__ __forceinline__ void attend_few(const AttentionArgs &a, int few_rows,
             if (a.window > 0 && from > 0) full_lo = (int)from;
         }
 
-        // `top` is the running maximum of the scores, the reference of `sum`. With codes the output has a reference of its own, the
-        // maximum of score + exponent of the V row: the weights 2^(score + exponent - base) are then at most 1, and fp16 loses only
-        // what is under 2^-25 of the largest contribution, however far the rows' exponents are apart.
+        // `top` is the running maximum of the scores, the reference of `sum` (with 16 bits 2^kLift times the sum of the weights). With codes
+        // the output has a reference of its own, the maximum of score + exponent of the V row: the weights 2^(score + exponent - base)
+        // are then at most 1 before the lift, however far the rows' exponents are apart.
         float acc[NT][kSteps][4];                 // elements (16 n + g8, + 8) or, with codes, (16 n + 2 g8, + 1) of rows 2c, 2c + 1
         float top[NT][2], base[NT][2], sum[NT][2];
 #pragma unroll
@@ -381,8 +385,8 @@ __device__ __forceinline__ void attend_few(const AttentionArgs &a, int few_rows,
                         if constexpr (kEight) u4 = fmaxf(u4, __shfl_xor_sync(0xFFFFFFFFu, u4, x));
                     }
                     const float now = fmaxf(top[m][j], t4);
-                    const float ref = now == -CUDART_INF_F ? 0.0f : now;       // nothing seen yet: every weight is exp2(-inf) = 0
-                    const float fall = exp2_fast(top[m][j] - ref);
+                    const float peak = now == -CUDART_INF_F ? 0.0f : now;      // nothing seen yet: every weight is exp2(-inf) = 0
+                    const float fall = exp2_fast(top[m][j] - peak), ref = kEight ? peak : peak - kLift;
                     if constexpr (!kEight) moved |= now != top[m][j];
                     top[m][j] = now;
                     alpha[j] = fall;
@@ -391,6 +395,7 @@ __device__ __forceinline__ void attend_few(const AttentionArgs &a, int few_rows,
                         const float high = fmaxf(base[m][j], u4);
                         above = high == -CUDART_INF_F ? 0.0f : high;
                         alpha[j] = exp2_fast(base[m][j] - above);
+                        above -= kLift;
                         moved |= high != base[m][j];
                         base[m][j] = high;
                     }
@@ -466,7 +471,8 @@ __device__ __forceinline__ void attend_few(const AttentionArgs &a, int few_rows,
                 for (int x = 4; x < 32; x <<= 1) l += __shfl_xor_sync(0xFFFFFFFFu, l, x);
                 const int r = m * 8 + 2 * c4 + j;
                 if (r < t.rows) {
-                    if (g8 == 0) stat[warp * kRows + r] = make_float4(top[m][j], l, kEight ? base[m][j] : top[m][j], 0.0f);
+                    if constexpr (!kEight) l *= pow2f(-(int)kLift);
+                    if (g8 == 0) stat[warp * kRows + r] = make_float4(top[m][j], l, (kEight ? base[m][j] : top[m][j]) - kLift, 0.0f);
                     float *dst = part + (warp * kRows + r) * kPart;
 #pragma unroll
                     for (int n = 0; n < kSteps; ++n) {

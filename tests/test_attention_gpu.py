@@ -637,3 +637,42 @@ def test_query_rows_at_the_top_of_bf16(gpu, bits, q_lens):
     qb = bits_of(mb.BFLOAT16, q)
     got = mb.paged_attention(mb.Tensor.from_bits(gpu, mb.BFLOAT16, qb), p.cache, p.batch).to_bits()
     check_attention(p, qb, got)
+
+
+@pytest.mark.parametrize("name,bits", [("fp16", 16), ("fp16", 8), ("bf16", 8), ("bf16", 16)])
+@pytest.mark.parametrize("q_lens,kv_lens", [([1], [30000]), ([8], [30000]), ([16], [30000]), ([20], [30000]), ([300], [900]), ([1, 20, 300], [700, 9000, 900])])
+@pytest.mark.parametrize("gap", [20.5, 24.7, 28.3])
+def test_many_small_weights_beside_a_large_one(gpu, name, bits, q_lens, kv_lens, gap):
+    """The first cached token's weight is 2^gap times that of every other one; all elements of the output but the first come from the
+    others, however small their weights are. fp16 weights under 2^-21 of the largest (of the tensor cores' tiles; 2^-29 in the streaming
+    kernel) are off by up to 2^-32 of it, the others by half a step."""
+    dt, dim = DTYPES[name], 16
+    p = Paged(gpu, dt, bits, q_lens, kv_lens, kv_heads=1, dim=dim, page=128, seed=15)
+    for b, n in enumerate(kv_lens):
+        k, v = np.zeros((n, dim)), np.ones((n, dim))
+        k[0, 0] = 16.0
+        v[0, 1:], v[1:, 0] = 0.0, 0.0
+        pos = np.arange(n)
+        at = np.asarray(p.tables[b])[pos // p.page], 0, pos % p.page
+        for side, rows in (("k", k), ("v", v)):
+            if bits == 8:
+                p.pool[side][at], p.exps[side][at] = A.quantise(rows, dt)
+            else:
+                p.pool[side][at] = bits_of(dt, rows)
+    p.upload()
+    tokens = sum(q_lens)
+    q = np.zeros((tokens, 2, dim))
+    q[:, :, 0] = 1.0
+    q[:, 1, 1] = 1.0
+    qb, scale = bits_of(dt, q), gap * np.log(2.0) / 16
+    lse = mb.Tensor(gpu, mb.FLOAT32, (tokens, 2))
+    out = mb.paged_attention(mb.Tensor.from_bits(gpu, dt, qb), p.cache, p.batch, lse=lse, scale=scale)
+    got = out.to_bits()
+    if gap > 21 and dt == mb.FLOAT16 and 2 * max(q_lens) > 32:
+        at = 0
+        for b, n in enumerate(q_lens):
+            want = A.attention(O.bits_to_f64(dt, qb[at:at + n]), p.rows("k", b), p.rows("v", b), scale, True, 0)[0]
+            assert (np.abs(O.bits_to_f64(dt, got[at:at + n]) - want) <= kv_lens[b] * 2.0 ** -32 + 2.0 ** -10 * want + 2.0 ** -25).all()
+            at += n
+    else:
+        check_attention(p, qb, got, lse.to_bits().view(np.float32).astype(np.float64), scale=scale)
