@@ -213,7 +213,8 @@ typedef struct magb200_kv_cache_t {
  * kv_len[b] counts its cached tokens INCLUDING its new ones, which are its last cu_q[b + 1] - cu_q[b]; a new token whose position
  * would be negative has no place. pages[b][i] is the page of positions i * page_size and up; sequences may share pages that
  * the call does not write. max_q and max_kv bound the new and cached tokens of any sequence (0: all rows / the whole table):
- * a sequence with more new tokens than max_q is an error, max_kv only steers how work is split. Device pointers. */
+ * a sequence with more new tokens than max_q is an error, max_kv only steers how work is split. Device pointers. A sequence whose
+ * own offsets do not fit is skipped as a whole; rows that offsets which do not ascend give to several sequences come from any of them. */
 typedef struct magb200_kv_batch_t {
     int32_t batch, max_pages;
     int32_t max_q, max_kv;

@@ -259,6 +259,17 @@ __device__ __forceinline__ Slot locate(const KvCache &c, const KvBatch &b, int s
     return s;
 }
 
+// Whether the offsets of a sequence fit: they ascend, stay within the rows and, of a write, hold at most max_q new tokens.
+template <bool kRead> __device__ __forceinline__ bool offsets_fit(const KvBatch &b, int64_t begin, int64_t end) {
+    return begin >= 0 && end >= begin && end <= b.tokens && (kRead || end - begin <= b.max_q);
+}
+// The threads of the grid look at all sequences' offsets, those that no token leads to among them. A function of its own: inside the
+// kernel it costs the moves behind it their schedule (write of 32768 tokens to 8 bits 42.5 us, so 45 to 46).
+template <bool kRead> __device__ __noinline__ void check_offsets(const KvBatch &b, const int32_t *cu) {
+    for (int64_t i = (int64_t)blockIdx.x * kRowThreads + threadIdx.x; i < b.batch; i += (int64_t)gridDim.x * kRowThreads)
+        if (!offsets_fit<kRead>(b, cu[i], cu[i + 1])) atomicOr(b.status + kBatchWord, kBadRows);
+}
+
 struct CacheMoveArgs {
     KvCache cache;
     KvBatch batch;
@@ -276,6 +287,7 @@ __global__ void __launch_bounds__(kRowThreads) kv_move_kernel(const __grid_const
     const int64_t first = (int64_t)blockIdx.x * a.per_cta;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const KvCache &c = a.cache;
+    if (blockIdx.x <= (unsigned)a.batch.batch / kRowThreads) check_offsets<kRead>(a.batch, a.cu);
     for (int i = warp; i < a.per_cta; i += kRowThreads / 32) {
         const int64_t t = first + i;
         Slot s;
@@ -283,7 +295,7 @@ __global__ void __launch_bounds__(kRowThreads) kv_move_kernel(const __grid_const
         if (t < a.batch.tokens) {
             const int seq = find_sequence(a.cu, a.batch.batch, t, lane);
             const int64_t begin = a.cu[seq], end = a.cu[seq + 1], kv = a.batch.kv_len[seq];
-            if (t >= begin && t < end) {      // rows behind the last sequence belong to nobody
+            if (t >= begin && t < end && offsets_fit<kRead>(a.batch, begin, end)) {      // rows behind the last sequence belong to nobody
                 const int64_t pos = kRead ? t - begin : kv - (end - t);
                 if (lane == 0) {
                     if (kRead && pos >= kv) atomicOr(a.batch.status + kBatchWord, kBadLength);   // more rows asked for than are cached

@@ -676,3 +676,111 @@ def test_many_small_weights_beside_a_large_one(gpu, name, bits, q_lens, kv_lens,
             at += n
     else:
         check_attention(p, qb, got, lse.to_bits().view(np.float32).astype(np.float64), scale=scale)
+
+
+def batch_of(gpu, cu, kv_lens, tables, max_q=0):
+    """A batch with offsets as they are, sound or not."""
+    width = max(len(t) for t in tables)
+    table = np.full((len(tables), width), -1, np.int32)
+    for b, t in enumerate(tables):
+        table[b, :len(t)] = t
+    return mb.KVBatch(len(tables), width, cu_q=DeviceArray(gpu, np.asarray(cu, np.int32)), kv_len=DeviceArray(gpu, np.asarray(kv_lens, np.int32)),
+                      pages=DeviceArray(gpu, table), max_q=max_q)
+
+
+BAD_OFFSETS = [([0, 3, 400], 0, [0]),                     # past the rows
+               ([0, 3, 43], 20, [0]),                     # more new tokens than max_q
+               ([0, 43, 3], 0, [0]),                      # descending
+               ([-2, 3, 43], 0, [1]),                     # before the rows
+               ([43, 43, 0], 0, []),                      # no row belongs to anyone
+               ([0, 0, 2 ** 31 - 1], 0, []), ([2 ** 31 - 1, -2 ** 31, 0], 0, [])]
+
+
+def reported(gpu, words):
+    with pytest.raises(mb.MagB200Error) as e:
+        mb.synchronize(gpu)
+    assert e.value.code == mb.ERR_INVALID_ARG and words in str(e.value)
+    mb.synchronize(gpu)                                                   # once
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("cu,max_q,sound", BAD_OFFSETS)
+def test_offsets_that_do_not_fit_are_reported_by_the_write(gpu, bits, cu, max_q, sound):
+    """The sequences in `sound` are written as they should be, the others not at all."""
+    p = Paged(gpu, mb.BFLOAT16, bits, [3, 40], [90, 100], kv_heads=2, dim=64, page=16, seed=5)
+    rows = bits_of(mb.BFLOAT16, np.random.default_rng(3).standard_normal((43, 2, 64)))
+    t = mb.Tensor.from_bits(gpu, mb.BFLOAT16, rows)
+    mb.kv_cache_write(p.cache, batch_of(gpu, cu, [90, 100], p.tables, max_q), t, t)
+    reported(gpu, "offsets")
+    want = {(n, "pool"): p.pool[n].copy() for n in ("k", "v")} | {(n, "exps"): p.exps[n].copy() for n in p.exps}
+    for b in sound:
+        for i in range(cu[b], cu[b + 1]):
+            pos = p.kv_lens[b] - (cu[b + 1] - i)
+            at = p.tables[b][pos // 16], slice(None), pos % 16
+            for n in ("k", "v"):
+                if bits == 8:
+                    want[n, "pool"][at], want[n, "exps"][at] = A.quantise(O.bits_to_f64(mb.BFLOAT16, rows[i]), mb.BFLOAT16)
+                else:
+                    want[n, "pool"][at] = rows[i]
+    got = p.download()
+    assert all(np.array_equal(got[key], w) for key, w in want.items())
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("cu,max_q,sound", [c for c in BAD_OFFSETS if not c[1]])
+def test_offsets_that_do_not_fit_are_reported_by_the_read(gpu, bits, cu, max_q, sound):
+    p = Paged(gpu, mb.BFLOAT16, bits, [3, 40], [90, 100], kv_heads=2, dim=64, page=16, seed=5)
+    before = np.full((43, 2, 64), 0x1234, np.uint16)
+    k, v = mb.Tensor.from_bits(gpu, mb.BFLOAT16, before), mb.Tensor.from_bits(gpu, mb.BFLOAT16, before)
+    mb.kv_cache_read(p.cache, p.batch, DeviceArray(gpu, np.asarray(cu, np.int32)), k, v)
+    reported(gpu, "offsets")
+    for name, t in (("k", k), ("v", v)):
+        want = before.copy()
+        for b in sound:
+            want[cu[b]:cu[b + 1]] = bits_of(mb.BFLOAT16, p.rows(name, b, cu[b + 1] - cu[b]))
+        assert np.array_equal(t.to_bits(), want)
+
+
+def test_bad_offsets_among_many_sequences_are_reported(gpu):
+    """A sequence without tokens of its own, far from every token's, with more sequences than the grid has threads."""
+    n = 2000
+    cu = np.zeros(n + 1, np.int32)
+    cu[1:] = 2
+    cu[1500] = 1                                                          # down and up again, within the rows
+    table = DeviceArray(gpu, np.zeros((n, 1), np.int32))
+    batch = mb.KVBatch(n, 1, cu_q=DeviceArray(gpu, cu), kv_len=DeviceArray(gpu, np.full(n, 2, np.int32)), pages=table)
+    cache = mb.KVCache(gpu, mb.BFLOAT16, 1, 16, 1, 16)
+    rows = mb.Tensor.from_bits(gpu, mb.BFLOAT16, np.zeros((2, 1, 16), np.uint16))
+    mb.kv_cache_write(cache, batch, rows, rows)
+    reported(gpu, "offsets")
+    out = mb.Tensor(gpu, mb.BFLOAT16, (2, 1, 16)), mb.Tensor(gpu, mb.BFLOAT16, (2, 1, 16))
+    mb.kv_cache_read(cache, batch, DeviceArray(gpu, cu), *out)
+    reported(gpu, "offsets")
+
+
+def test_pages_and_lengths_that_do_not_fit_are_reported_by_write_and_read(gpu):
+    """A bad page that a write or a read has to touch, and more rows asked for than are cached: the rest is done."""
+    p = Paged(gpu, mb.BFLOAT16, 16, [3, 40], [90, 100], kv_heads=2, dim=64, page=16, seed=5)
+    rows = bits_of(mb.BFLOAT16, np.random.default_rng(3).standard_normal((43, 2, 64)))
+    t = mb.Tensor.from_bits(gpu, mb.BFLOAT16, rows)
+    tables = [list(x) for x in p.tables]
+    tables[1][4] = 10 ** 6                                                # positions 64 .. 79 of sequence 1, whose new tokens are 60 .. 99
+    want = p.pool["k"].copy()
+    for i in range(43):
+        b, pos = (0, 87 + i) if i < 3 else (1, 57 + i)
+        if not (b == 1 and 64 <= pos < 80):
+            want[p.tables[b][pos // 16], :, pos % 16] = rows[i]
+    mb.kv_cache_write(p.cache, batch_of(gpu, [0, 3, 43], [90, 100], tables), t, t)
+    reported(gpu, "a page")
+    assert np.array_equal(p.download()["k", "pool"], want)
+    p.pool["k"] = want
+    before = np.full((200, 2, 64), 0x1234, np.uint16)
+    for bad, cu, words in ((tables, [0, 90, 190], "a page"), (p.tables, [0, 90, 195], "a length")):
+        k, v = mb.Tensor.from_bits(gpu, mb.BFLOAT16, before), mb.Tensor.from_bits(gpu, mb.BFLOAT16, before)
+        mb.kv_cache_read(p.cache, batch_of(gpu, [0, 3, 43], [90, 100], bad), DeviceArray(gpu, np.asarray(cu, np.int32)), k, v)
+        reported(gpu, words)
+        expect = before.copy()
+        expect[:190] = np.concatenate([bits_of(mb.BFLOAT16, p.rows("k", 0, 90)), bits_of(mb.BFLOAT16, p.rows("k", 1, 100))])
+        if bad is tables:
+            expect[90 + 64:90 + 80] = 0x1234
+        assert np.array_equal(k.to_bits(), expect)
