@@ -211,7 +211,7 @@ typedef struct magb200_kv_cache_t {
 /* The sequences of a call. New tokens are packed: sequence b owns rows cu_q[b] .. cu_q[b + 1] - 1 of q, k, v and out (cu_q[0]
  * = 0, ascending, equal for a sequence without new tokens; rows from cu_q[batch] on belong to nobody and are left alone).
  * kv_len[b] counts its cached tokens INCLUDING its new ones, which are its last cu_q[b + 1] - cu_q[b]; a new token whose position
- * would be negative has no place. pages[b][i] is the page of positions i * page_size and up; sequences may share pages that
+ * would be negative has no place. A negative kv_len is an error if the sequence has new tokens, and counts as 0. pages[b][i] is the page of positions i * page_size and up; sequences may share pages that
  * the call does not write. max_q and max_kv bound the new and cached tokens of any sequence (0: all rows / the whole table):
  * a sequence with more new tokens than max_q is an error, max_kv only steers how work is split. Device pointers. A sequence whose
  * own offsets do not fit is skipped as a whole; rows that offsets which do not ascend give to several sequences come from any of them. */

@@ -26,9 +26,13 @@ __device__ __forceinline__ bool sequence_of(const AttentionArgs &a, int b, Tile 
     const int room = table > 0x7FFFF000 ? 0x7FFFF000 : (int)table;       // positions fit 32 bits with room for a block
     if (begin < 0 || end < begin || end > a.batch.tokens || end - begin > a.batch.max_q) { atomicOr(a.batch.status + kBatchWord, kBadRows); return false; }
     if (kv > room) { atomicOr(a.batch.status + kBatchWord, kBadLength); kv = room; }
+    if (kv < 0) {
+        if (end > begin) atomicOr(a.batch.status + kBatchWord, kBadLength);
+        kv = 0;
+    }
     t.q_begin = begin;
     t.q_len = end - begin;
-    t.kv_len = kv < 0 ? 0 : kv;
+    t.kv_len = kv;
     t.rows = t.q_len * a.group;
     return t.q_len > 0;
 }

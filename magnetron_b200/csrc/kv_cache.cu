@@ -246,11 +246,14 @@ constexpr int kMaxTokensPerCta = 16;
 struct Slot { int64_t page; int offset; };   // page < 0: nothing to do for this token
 
 // The page and slot of position `pos` of sequence b. Bounds are checked here: what does not fit raises the word and is skipped.
-__device__ __forceinline__ Slot locate(const KvCache &c, const KvBatch &b, int seq, int64_t pos) {
+__device__ __forceinline__ Slot locate(const KvCache &c, const KvBatch &b, int seq, int64_t kv, int64_t pos) {
     Slot s;
     s.page = -1;
     s.offset = (int)(pos & (c.page_size - 1));
-    if (pos < 0) return s;                    // fewer cached tokens than new ones: this one has no place
+    if (pos < 0) {                            // fewer cached tokens than new ones: this one has no place
+        if (kv < 0) atomicOr(b.status + kBatchWord, kBadLength);
+        return s;
+    }
     const int64_t entry = pos >> c.page_shift;
     if (entry >= b.max_pages) { atomicOr(b.status + kBatchWord, kBadLength); return s; }
     const int32_t page = b.table[(int64_t)seq * b.max_pages + entry];
@@ -299,7 +302,7 @@ __global__ void __launch_bounds__(kRowThreads) kv_move_kernel(const __grid_const
                 const int64_t pos = kRead ? t - begin : kv - (end - t);
                 if (lane == 0) {
                     if (kRead && pos >= kv) atomicOr(a.batch.status + kBatchWord, kBadLength);   // more rows asked for than are cached
-                    else s = locate(c, a.batch, seq, pos);
+                    else s = locate(c, a.batch, seq, kv, pos);
                 }
             }
         }

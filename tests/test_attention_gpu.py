@@ -784,3 +784,32 @@ def test_pages_and_lengths_that_do_not_fit_are_reported_by_write_and_read(gpu):
         if bad is tables:
             expect[90 + 64:90 + 80] = 0x1234
         assert np.array_equal(k.to_bits(), expect)
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("q_lens", [[2, 1], [2, 70]])
+def test_negative_lengths_are_reported(gpu, bits, q_lens):
+    """A sequence with new tokens and a negative length: reported by all operators; its rows see nothing, the others are as ever. Without
+    new tokens its length is nobody's business."""
+    p = Paged(gpu, mb.BFLOAT16, bits, q_lens, [90, 100], kv_heads=2, dim=64, page=16, seed=5)
+    tokens = sum(q_lens)
+    rows = mb.Tensor.from_bits(gpu, mb.BFLOAT16, bits_of(mb.BFLOAT16, np.random.default_rng(3).standard_normal((tokens, 2, 64))))
+    q = mb.Tensor.from_bits(gpu, mb.BFLOAT16, bits_of(mb.BFLOAT16, np.random.default_rng(4).standard_normal((tokens, 4, 64))))
+    want = mb.paged_attention(q, p.cache, p.batch).to_bits()
+    cu = [0, q_lens[0], tokens]
+    bad = batch_of(gpu, cu, [90, -3], p.tables)
+    out = mb.paged_attention(q, p.cache, bad)
+    reported(gpu, "a length")
+    got = out.to_bits()
+    assert np.array_equal(got[:q_lens[0]], want[:q_lens[0]]) and (got[q_lens[0]:] == 0).all()
+    before = p.download()
+    mb.kv_cache_write(p.cache, batch_of(gpu, cu, [-1, -3], p.tables), rows, rows)
+    reported(gpu, "a length")
+    after = p.download()
+    assert all(np.array_equal(before[key], after[key]) for key in before)
+    mb.kv_cache_read(p.cache, bad, DeviceArray(gpu, np.array([0, 0, 1], np.int32)), rows, mb.Tensor(gpu, mb.BFLOAT16, (tokens, 2, 64)))
+    reported(gpu, "a length")
+    idle = batch_of(gpu, [0, tokens, tokens], [90, -3], p.tables)
+    mb.kv_cache_write(p.cache, idle, rows, rows)
+    mb.paged_attention(q, p.cache, idle, mb.Tensor(gpu, mb.BFLOAT16, (tokens, 4, 64)))
+    mb.synchronize(gpu)
