@@ -164,12 +164,30 @@ __global__ void __launch_bounds__(kRowThreads, 4) qk_norm_rope_kernel(const __gr
             for (int j = 0; j < kRun; ++j) xa[j] = xb[j] = 0.0f;
             if (mine) load_runs<DT, kRun, kVec>(src.p, (first + token) * src.token_stride + h * src.head_stride, u, a.rope, at, xa, xb);
             if (weight) {
-                float sum = 0.0f;
+                auto mean = [&](float by, float eps) {                     // of the squares of by * x, over all the row's lanes, and eps
+                    float sum = 0.0f;
 #pragma unroll
-                for (int j = 0; j < kRun; ++j) sum = fmaf(xa[j], xa[j], fmaf(xb[j], xb[j], sum));
+                    for (int j = 0; j < kRun; ++j) {
+                        const float p = xa[j] * by, q = xb[j] * by;
+                        sum = fmaf(p, p, fmaf(q, q, sum));
+                    }
 #pragma unroll
-                for (int m = LPR / 2; m > 0; m >>= 1) sum += __shfl_xor_sync(lanes, sum, m);
-                const float inv = rsqrtf(fmaf(sum, inv_dim, a.eps));
+                    for (int m = LPR / 2; m > 0; m >>= 1) sum += __shfl_xor_sync(lanes, sum, m);
+                    return fmaf(sum, inv_dim, eps);
+                };
+                const float square = mean(1.0f, a.eps);
+                float inv = rsqrtf(square);
+                // squares past the range of fp32, or so small that they lose bits, are taken again of the row times a power of two; it goes
+                // to the root of large rows and to the elements of small ones, which loses nothing of either
+                if (!(square >= 0x1p-100f && square <= 3.4028235e38f)) {
+                    const bool small = square < 1.0f;
+                    const float by = small ? 0x1p96f : 0x1p-70f;
+                    inv = rsqrtf(mean(by, a.eps * by * by));
+                    if (!small) inv *= by;
+#pragma unroll
+                    for (int j = 0; j < kRun; ++j)
+                        if (small) { xa[j] *= by; xb[j] *= by; }
+                }
                 if (mine) {
 #pragma unroll
                     for (int j = 0; j < kRun; ++j) { xa[j] = xa[j] * inv * ga[j]; xb[j] = xb[j] * inv * gb[j]; }

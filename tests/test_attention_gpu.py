@@ -813,3 +813,34 @@ def test_negative_lengths_are_reported(gpu, bits, q_lens):
     mb.kv_cache_write(p.cache, idle, rows, rows)
     mb.paged_attention(q, p.cache, idle, mb.Tensor(gpu, mb.BFLOAT16, (tokens, 4, 64)))
     mb.synchronize(gpu)
+
+
+@pytest.mark.parametrize("name", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("dim", [8, 64, 96, 128, 256])
+@pytest.mark.parametrize("pad", [0, 1])
+def test_norm_of_rows_whose_squares_leave_fp32(gpu, name, dim, pad):
+    """Rows so large or so small that the squares of their elements overflow or underflow, beside ordinary ones."""
+    dt = DTYPES[name]
+    rng = np.random.default_rng(dim)
+    powers = {"fp16": [15, 0, -14, -20, -24]}.get(name, [126, 100, 64, 63, 0, -40, -50, -51, -64, -100, -126, -140 if name == "fp32" else -130])
+    x = rng.uniform(1.0, 1.9, (len(powers) + 1, 3, dim)) * rng.choice([-1.0, 1.0], (len(powers) + 1, 3, dim))
+    x[:-1] *= np.exp2(np.asarray(powers, np.float64))[:, None, None]
+    x[:, 1, 1:] *= 2.0 ** -9                                               # one element makes the mean
+    x[-1, 2] = 0.0
+    buf = np.zeros((len(powers) + 1, 3 * dim + pad), np.uint32 if dt == mb.FLOAT32 else np.uint16)
+    buf[:, pad:] = bits_of(dt, x).reshape(len(powers) + 1, -1)
+    t = mb.Tensor.from_bits(gpu, dt, buf).as_strided((len(powers) + 1, 3, dim), (3 * dim + pad, dim, 1), pad)
+    w = bits_of(dt, rng.uniform(0.5, 1.5, dim))
+    given = O.bits_to_f64(dt, bits_of(dt, x))
+    for eps in (1e-6, 0.0, 1.0):
+        got = O.bits_to_f64(dt, mb.qk_norm_rope(t, None, None, q_weight=mb.Tensor.from_bits(gpu, dt, w), eps=eps)[0].to_bits())
+        eps32 = np.float64(np.float32(eps))
+        with np.errstate(invalid="ignore"):
+            want = A.norm_rope(given, O.bits_to_f64(dt, w), eps32, None, None, 0, False, 1.0)[0]
+        # one rounding of the result; the mean of squares, its root and the products: dim + 32 roundings of fp32; where they are
+        # subnormal half a step of fp32 for each of the two products, the first times a weight below 1.5, and half one of the result
+        least = {"fp16": 2.0 ** -25, "bf16": 2.0 ** -134, "fp32": 0.0}[name] + 2.5 * 2.0 ** -150
+        tol = HALF_STEP[dt] * np.abs(want) + (dim + 32) * 2.0 ** -24 * np.abs(want) + least
+        some = np.isfinite(want)                                          # a row of zeros with eps 0 has no norm
+        assert np.isfinite(got[some]).all() and (np.abs(got - want)[some] <= tol[some]).all(), (eps, np.argwhere(~(np.abs(got - want) <= tol))[:4].tolist())
+        assert some[:-1].all() and np.isnan(got[~some]).all()
