@@ -55,6 +55,14 @@ def _pointer(x, dtype, count: int, what: str):
     return x.ptr
 
 
+def _device_of(arrays):
+    """The device of those that are DeviceArrays; None if none is."""
+    devices = {x.device for x in arrays if isinstance(x, DeviceArray)}
+    if len(devices) > 1:
+        raise ValueError(f"arrays of the devices {sorted(devices)} in one header")
+    return devices.pop() if devices else None
+
+
 class KVCache:
     """A paged KV cache (magb200_kv_cache_t): K and V pools of [pages][kv_heads][page_size][head_dim], with bits=8 e4m3 codes and
     an exponent per row. Pools are allocated, uninitialised, unless device pointers are given."""
@@ -92,6 +100,7 @@ class KVBatch:
 
     def __init__(self, batch: int, max_pages: int, *, cu_q, kv_len, pages, max_q: int = 0, max_kv: int = 0):
         self.arrays = (cu_q, kv_len, pages)
+        self.device = _device_of(self.arrays)               # of arrays that are no plain pointers
         self.struct = KVBatchStruct(batch, max_pages, max_q, max_kv, _pointer(cu_q, np.int32, batch + 1, "cu_q"),
                                     _pointer(kv_len, np.int32, batch, "kv_len"), _pointer(pages, np.int32, batch * max_pages, "pages"))
         self.header = C.byref(self.struct)
@@ -114,6 +123,7 @@ class Rope:
 
     def __init__(self, positions, inv_freq, rotary_dim: int, *, interleaved: bool = False, factor: float = 1.0):
         self.arrays = (positions, inv_freq)
+        self.device = _device_of(self.arrays)
         self.struct = RopeStruct(_pointer(positions, np.int32, 0, "positions"), _pointer(inv_freq, np.float32, rotary_dim // 2, "inv_freq"),
                                  rotary_dim, int(interleaved), factor, 0)
         self.header = C.byref(self.struct)
@@ -123,7 +133,7 @@ class Rope:
 # A decode step makes these calls once per layer and token, so they do nothing but pass headers on: the arguments' structs are made
 # once, the functions are looked up once, and the status is compared here.
 _bound = {}
-_APART = "the tensors of a call lie on one device"
+_APART = "the tensors and arrays of a call lie on one device"
 
 
 def _call(name: str, *args) -> None:
@@ -144,7 +154,7 @@ def qk_norm_rope(q: Tensor, k: Tensor | None, rope: Rope | None, q_out: Tensor |
         k_out = Tensor(k.device, k.dtype, k.shape)
     d = q.device
     if q_out.device != d or (k is not None and (k.device != d or k_out.device != d)) or (q_weight is not None and q_weight.device != d) or (
-            k_weight is not None and k_weight.device != d):
+            k_weight is not None and k_weight.device != d) or (rope is not None and rope.device not in (None, d)):
         raise ValueError(_APART)
     if rope is not None and rope.tokens < q.shape[0]:
         raise ValueError(f"qk_norm_rope: {rope.tokens} positions for {q.shape[0]} tokens")
@@ -155,14 +165,15 @@ def qk_norm_rope(q: Tensor, k: Tensor | None, rope: Rope | None, q_out: Tensor |
 
 def kv_cache_write(cache: KVCache, batch: KVBatch, k: Tensor, v: Tensor) -> None:
     """Puts the rows of the batch's new tokens into the cache."""
-    if not cache.device == k.device == v.device:
+    if not cache.device == k.device == v.device or batch.device not in (None, cache.device):
         raise ValueError(_APART)
     _call("magb200_kv_cache_write", cache.device, cache.header, batch.header, k.header(), v.header())
 
 
 def kv_cache_read(cache: KVCache, batch: KVBatch, cu_kv, k: Tensor, v: Tensor) -> None:
     """Fills rows cu_kv[b] .. cu_kv[b + 1] - 1 of k and v with the first cached tokens of sequence b."""
-    if not cache.device == k.device == v.device:
+    if not cache.device == k.device == v.device or batch.device not in (None, cache.device) or (
+            isinstance(cu_kv, DeviceArray) and cu_kv.device != cache.device):
         raise ValueError(_APART)
     _call("magb200_kv_cache_read", cache.device, cache.header, batch.header, _pointer(cu_kv, np.int32, batch.struct.batch + 1, "cu_kv"), k.header(), v.header())
 
@@ -172,7 +183,7 @@ def paged_attention(q: Tensor, cache: KVCache, batch: KVBatch, out: Tensor | Non
     """softmax(scale * q K^T + mask) V of the batch's new tokens over their cached ones; scale is head_dim ** -0.5 unless given."""
     if out is None:
         out = Tensor(q.device, q.dtype, q.shape)
-    if not cache.device == q.device == out.device or (lse is not None and lse.device != q.device):
+    if not cache.device == q.device == out.device or (lse is not None and lse.device != q.device) or batch.device not in (None, q.device):
         raise ValueError(_APART)
     _call("magb200_paged_attention", cache.device, q.header(), cache.header, batch.header, cache.scale if scale is None else scale, causal, window,
           out.header(), lse and lse.header())

@@ -241,3 +241,31 @@ def test_addresses_between_two_elements_are_refused():
         refused_address(mb.qk_norm_rope, tensor(Q, dtype), None, None, tensor(Q, dtype, at=FAR), q_weight=tensor((64,), dtype, at=16 * FAR + at - BASE))
     for rope in (mb.Rope(by_two, BASE, 64), mb.Rope(BASE, by_two, 64)):
         refused_address(mb.qk_norm_rope, tensor(Q), None, rope, out, q_weight=w)
+
+
+def test_arrays_of_another_device_are_refused():
+    """What a kernel would read of another device's memory: offsets, lengths, tables, positions and frequencies."""
+    rows, far = tensor((6, 2, 64)), tensor((6, 2, 64), at=FAR)
+
+    def there(**kw):
+        return mb.KVBatch(2, 4, **(dict(cu_q=array([0, 1, 2]), kv_len=array([1, 1]), pages=array(np.zeros((2, 4)))) | kw))
+
+    one = dict(cu_q=array([0, 1, 2], device=1), kv_len=array([1, 1], device=1), pages=array(np.zeros((2, 4)), device=1))
+    for name in one:
+        with pytest.raises(ValueError):
+            there(**{name: one[name]})                                       # arrays of two devices in one batch
+    with pytest.raises(ValueError):
+        mb.Rope(array(np.arange(6)), array(np.ones(32), np.float32, device=1), 64)
+    elsewhere, plain = there(**one), mb.KVBatch(2, 4, cu_q=BASE, kv_len=one["kv_len"], pages=BASE)
+    rope = mb.Rope(array(np.arange(6), device=1), array(np.ones(32), np.float32, device=1), 64)
+    for b in (elsewhere, plain):
+        for call in (lambda: mb.kv_cache_write(cache(), b, rows, rows), lambda: mb.kv_cache_read(cache(), b, BASE, rows, far),
+                     lambda: mb.paged_attention(tensor(Q), cache(), b, tensor(Q, at=FAR))):
+            with pytest.raises(ValueError, match="one device"):
+                call()
+    with pytest.raises(ValueError, match="one device"):
+        mb.kv_cache_read(cache(), there(), array([0, 1, 2], device=1), rows, far)
+    with pytest.raises(ValueError, match="one device"):
+        mb.qk_norm_rope(tensor(Q), None, rope, tensor(Q, at=FAR))
+    if mb.device_count() == 0:
+        refused(mb.ERR_NO_DEVICE, mb.kv_cache_write, cache(), batch(), rows, rows)    # plain pointers: nothing is known of them
