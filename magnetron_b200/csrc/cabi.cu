@@ -1282,7 +1282,8 @@ int magb200_paged_attention(int device, const magb200_view_t *q, const magb200_k
         if (((uintptr_t)rows[i]->p & 15u) || rows[i]->token_stride % 8 || rows[i]->head_stride % 8) { set_error("paged_attention: rows of q and of the result start on 16-byte boundaries"); return MAGB200_ERR_INVALID_ARG; }
     if (!rows_apart(out) || !rows_disjoint(out, q)) { set_error("paged_attention: the result overlaps itself or q"); return MAGB200_ERR_INVALID_ARG; }
     if (in_pools(a.cache, view_range(out))) { set_error("paged_attention: the result lies in the cache"); return MAGB200_ERR_INVALID_ARG; }
-    if (!isfinite(scale)) { set_error("paged_attention: scale is not finite"); return MAGB200_ERR_INVALID_ARG; }
+    a.scale_log2 = (float)(scale * 1.4426950408889634);
+    if (!isfinite(a.scale_log2)) { set_error("paged_attention: scale is not finite in 32 bits"); return MAGB200_ERR_INVALID_ARG; }
     if (window < 0 || (window > 0 && !causal)) { set_error("paged_attention: a window goes with a causal mask and is not negative"); return MAGB200_ERR_INVALID_ARG; }
     if (lse) {
         if ((rc = check_view(lse, "paged_attention lse"))) return rc;
@@ -1297,7 +1298,6 @@ int magb200_paged_attention(int device, const magb200_view_t *q, const magb200_k
         a.lse = (float *)view_data(lse);
     }
     a.group = (int)(q->shape[1] / a.cache.kv_heads);
-    a.scale_log2 = (float)(scale * 1.4426950408889634);
     a.causal = causal != 0;
     a.window = window > INT32_MAX ? 0 : window;                        // positions fit 32 bits: none falls out of such a window
     DeviceState *d;

@@ -269,3 +269,9 @@ def test_arrays_of_another_device_are_refused():
         mb.qk_norm_rope(tensor(Q), None, rope, tensor(Q, at=FAR))
     if mb.device_count() == 0:
         refused(mb.ERR_NO_DEVICE, mb.kv_cache_write, cache(), batch(), rows, rows)    # plain pointers: nothing is known of them
+
+
+@pytest.mark.parametrize("scale", [1e300, -1e39, 3e38])
+def test_scales_past_fp32_are_refused(scale):
+    """3e38 * log2(e), the factor of the scores, is past the largest number too."""
+    assert "32 bits" in refused(mb.ERR_INVALID_ARG, mb.paged_attention, tensor(Q), cache(), batch(), tensor(Q, at=FAR), scale=scale)
