@@ -191,8 +191,10 @@ int  magb200_matmul_grouped(int device, const magb200_view_t *x, int count, cons
  * Head norm with the rotation of positions, a paged KV cache as it is written and read back, and the attention of new tokens
  * over it: what the Qwen3 block does between its matmuls with RMSNorm, the rotation, CAT (the KV append), the scores matmul,
  * scale, mask, softmax and the P.V matmul (examples/qwen3/model.py:106-141). Device arrays of a batch are plain pointers; they
- * are read by the kernels, which check them: a page, an offset or a length that does not fit is skipped (nothing is read or
- * written out of range) and the next magb200_synchronize / magb200_download reports MAGB200_ERR_INVALID_ARG.
+ * are read by the kernels, which check them: nothing is read or written out of range, and what does not fit is reported by the next
+ * magb200_synchronize / magb200_download as MAGB200_ERR_INVALID_ARG. A sequence with offsets that do not fit is left out; rows in a
+ * page outside the cache are not written and not read (the attention takes them for rows of zeros); a length beyond the table
+ * is cut to it.
  * None of them allocates after its first call on a device, so all can be recorded into graphs (call the attention once first). */
 
 /* Paged KV cache: `pages` pages of `page_size` tokens (a power of two, 16 or more), one pool for K and one for V, each

@@ -11,7 +11,7 @@
 
 namespace magb200 {
 
-// Bits of the device word a kernel raises when it meets a table or a length that does not fit; the access is skipped.
+// Bits of the device word a kernel raises when it meets a table or a length that does not fit; nothing is read or written through it.
 constexpr int kBatchWord = 2;                // word of the status buffer
 constexpr int kWorkWord = 16;                // two words: work handed out by the running many-row kernel, its CTAs that have ended
 constexpr int kBadPage = 1, kBadRows = 2, kBadLength = 4;

@@ -290,7 +290,7 @@ static int check_status_word(DeviceState &d) {
     }
     if (h[kBatchWord] != 0) {
         MAGB200_CUDA_TRY(cudaMemsetAsync(d.status + kBatchWord, 0, sizeof(int), d.stream));
-        set_error("paged cache:%s%s%s; what did not fit was skipped", h[kBatchWord] & kBadPage ? " a page outside the cache" : "",
+        set_error("paged cache:%s%s%s; what did not fit was neither read nor written", h[kBatchWord] & kBadPage ? " a page outside the cache" : "",
                   h[kBatchWord] & kBadRows ? " offsets that do not ascend, pass the rows or exceed max_q" : "",
                   h[kBatchWord] & kBadLength ? " a length that is negative or beyond the block table or the cached tokens" : "");
         return MAGB200_ERR_INVALID_ARG;

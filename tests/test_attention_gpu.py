@@ -844,3 +844,25 @@ def test_norm_of_rows_whose_squares_leave_fp32(gpu, name, dim, pad):
         some = np.isfinite(want)                                          # a row of zeros with eps 0 has no norm
         assert np.isfinite(got[some]).all() and (np.abs(got - want)[some] <= tol[some]).all(), (eps, np.argwhere(~(np.abs(got - want) <= tol))[:4].tolist())
         assert some[:-1].all() and np.isnan(got[~some]).all()
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("q_lens", [[1, 2], [3, 70]])
+def test_attention_takes_rows_of_a_bad_page_for_zeros(gpu, bits, q_lens):
+    p = Paged(gpu, mb.BFLOAT16, bits, q_lens, [90, 200], kv_heads=2, dim=64, page=16, seed=5)
+    tables = [list(t) for t in p.tables]
+    tables[0][1], tables[1][9] = 10 ** 6, -7
+    for b, i in ((0, 1), (1, 9)):
+        for n in ("k", "v"):
+            p.pool[n][p.tables[b][i]] = 0
+            if bits == 8:
+                p.exps[n][p.tables[b][i]] = 0
+    p.upload()
+    tokens = sum(q_lens)
+    qb = bits_of(mb.BFLOAT16, np.random.default_rng(4).standard_normal((tokens, 4, 64)))
+    q, lse, want_lse = mb.Tensor.from_bits(gpu, mb.BFLOAT16, qb), mb.Tensor(gpu, mb.FLOAT32, (tokens, 4)), mb.Tensor(gpu, mb.FLOAT32, (tokens, 4))
+    want = mb.paged_attention(q, p.cache, p.batch, lse=want_lse).to_bits()
+    check_attention(p, qb, want)
+    got = mb.paged_attention(q, p.cache, batch_of(gpu, [0, q_lens[0], tokens], [90, 200], tables), lse=lse)
+    reported(gpu, "a page")
+    assert np.array_equal(got.to_bits(), want) and np.array_equal(lse.to_bits(), want_lse.to_bits())
