@@ -79,7 +79,8 @@ int  magb200_synchronize(int device);
  * on `device`; NULL restores the library's own stream. */
 int  magb200_set_stream(int device, void *cuda_stream);
 void *magb200_get_stream(int device);
-/* Cap the number of CTAs the tensor-core matmuls launch on `device` (0 = all 148 SMs). A tensor-parallel caller leaves a
+/* Cap the number of CTAs the tensor-core matmuls and the tensor-core attention (sequences of more than 32 (new token, query head)
+ * rows a KV head) launch on `device` (0 = all 148 SMs; the streaming kernels of decode steps take all). A tensor-parallel caller leaves a
  * few SMs free this way so that a collective running on another stream makes progress beside the persistent GEMM. */
 int  magb200_set_cta_limit(int device, int max_ctas);
 

@@ -60,6 +60,7 @@ struct AttentionArgs {
     float scale_log2;                        // scale * log2(e)
     int causal;
     int64_t window;                          // 0: none
+    int ctas;                                // multiprocessors that the tensor-core kernel may take
     float *partial;                          // workspace of split sequences
     size_t partial_bytes;
     int *arrived;                            // kMaxFewCtas words, zero between launches: parts done of the pair that begins in a CTA

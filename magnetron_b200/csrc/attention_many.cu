@@ -819,14 +819,14 @@ template <int DT> int launch_all(const ManyArgs &m, int ctas, cudaStream_t st, b
     if (m.a.cache.bits == 8) return m.a.cache.dim <= 64 ? launch<DT, true, 64>(m, ctas, st, early) : launch<DT, true, 128>(m, ctas, st, early);
     return m.a.cache.dim <= 64 ? launch<DT, false, 64>(m, ctas, st, early) : launch<DT, false, 128>(m, ctas, st, early);
 }
-ManyArgs many_args(const AttentionArgs &a, const AttentionPlan &p, int sms) {
+ManyArgs many_args(const AttentionArgs &a, const AttentionPlan &p) {
     ManyArgs m;
     m.a = a; m.few_rows = p.few_rows;
     // A unit that is cut has more than 2 kLeastBlocks blocks; fewer than 2 parts for every CTA have to be held. From two rounds on the
     // queue alone keeps the multiprocessors busy, and the second kernel costs what cutting the rest saves (a prefill of 8 x 2048 tokens:
     // 409 us, 417 with its last 136 units in parts).
-    const size_t parts = (size_t)sms * 2 * kManyRows * (a.cache.dim + 4) * sizeof(float);
-    m.split = p.many_tiles * a.cache.kv_heads < 2 * sms && p.many_keys > 2 * kLeastBlocks * kBlock && parts + sms * sizeof(CutUnit) <= a.partial_bytes;
+    const size_t parts = (size_t)a.ctas * 2 * kManyRows * (a.cache.dim + 4) * sizeof(float);
+    m.split = p.many_tiles * a.cache.kv_heads < 2 * a.ctas && p.many_keys > 2 * kLeastBlocks * kBlock && parts + a.ctas * sizeof(CutUnit) <= a.partial_bytes;
     m.cut_units = reinterpret_cast<CutUnit *>(reinterpret_cast<char *>(a.partial) + parts);
     m.tiles = (int)p.many_tiles;
     m.beside = p.few_ctas > 0;
@@ -839,17 +839,15 @@ ManyArgs many_args(const AttentionArgs &a, const AttentionPlan &p, int sms) {
 }  // namespace
 
 int launch_attend_many(const AttentionArgs &a, const AttentionPlan &p, cudaStream_t st, bool early) {
-    const int sms = num_sms();
-    const ManyArgs m = many_args(a, p, sms);
+    const ManyArgs m = many_args(a, p);
     const int64_t units = p.many_tiles * a.cache.kv_heads;
-    const int ctas = m.split || units > sms ? sms : (int)units;
+    const int ctas = m.split || units > a.ctas ? a.ctas : (int)units;
     return a.cache.dtype == MAGB200_BF16 ? launch_all<MAGB200_BF16>(m, ctas, st, early) : launch_all<MAGB200_F16>(m, ctas, st, early);
 }
 int launch_join_many(const AttentionArgs &a, const AttentionPlan &p, cudaStream_t st) {
-    const int sms = num_sms();
-    const ManyArgs m = many_args(a, p, sms);
+    const ManyArgs m = many_args(a, p);
     if (!m.split) return MAGB200_OK;
-    const dim3 grid((unsigned)sms, kManyRows / 32);
+    const dim3 grid((unsigned)a.ctas, kManyRows / 32);
     const CutUnit *units = m.cut_units;
     return a.cache.dtype == MAGB200_BF16 ? launch_kernel(join_kernel<MAGB200_BF16>, grid, kJoinThreads, 0, st, true, a, units)
                                          : launch_kernel(join_kernel<MAGB200_F16>, grid, kJoinThreads, 0, st, true, a, units);

@@ -91,7 +91,7 @@ struct DeviceState {
     size_t staging_bytes[3] = {0, 0, 0};
     char name[256] = "";
     bool capturing = false;          // between graph_begin_capture and graph_end_capture
-    int cta_limit = 0;               // 0: all SMs; else the tensor-core GEMMs launch at most this many CTAs
+    int cta_limit = 0;               // 0: all SMs; else the tensor-core GEMMs and the tensor-core attention launch at most this many CTAs
     cudaStream_t h2d_stream = nullptr;   // copy streams of the overlapped transfers (created on first use)
     cudaStream_t d2h_stream = nullptr;
     bool d2h_pending = false;            // overlapped downloads submitted since the last synchronize
@@ -1317,6 +1317,7 @@ int magb200_paged_attention(int device, const magb200_view_t *q, const magb200_k
         d->chain_open = false;
     }
     a.batch.status = d->status;
+    a.ctas = d->cta_limit > 0 ? d->cta_limit : num_sms();
     a.partial = d->attention_parts;
     a.partial_bytes = attention_workspace_bytes();
     a.arrived = (int *)((char *)d->attention_parts + attention_workspace_bytes());

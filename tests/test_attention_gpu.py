@@ -1,5 +1,6 @@
 """Head norm + rotation, the paged KV cache and attention over it, on the device against the 64-bit definitions."""
 import ctypes as C
+import time
 
 import numpy as np
 import pytest
@@ -866,3 +867,41 @@ def test_attention_takes_rows_of_a_bad_page_for_zeros(gpu, bits, q_lens):
     got = mb.paged_attention(q, p.cache, batch_of(gpu, [0, q_lens[0], tokens], [90, 200], tables), lse=lse)
     reported(gpu, "a page")
     assert np.array_equal(got.to_bits(), want) and np.array_equal(lse.to_bits(), want_lse.to_bits())
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("limit", [1, 3, 20, 147])
+def test_attention_under_a_limit_of_ctas(gpu, bits, limit):
+    """Units whole and in parts, beside single tokens, on fewer multiprocessors than there are."""
+    L = mb.lib()
+    mb.check(L.magb200_set_cta_limit(gpu, limit))
+    try:
+        for q_lens, kv_lens, heads, hk in (([330, 1, 40, 700], [2500, 900, 4000, 1400], 6, 2), ([200], [3300], 8, 1), ([50] * 8, [1300] * 8, 16, 8)):
+            attend(gpu, Paged(gpu, mb.BFLOAT16, bits, q_lens, kv_lens, kv_heads=hk, dim=64, page=32, seed=limit), heads)
+    finally:
+        mb.check(L.magb200_set_cta_limit(gpu, 0))
+
+
+def test_the_attention_leaves_multiprocessors_free(gpu):
+    """The limit of CTAs shows in the time: 128 units on four multiprocessors, so on all of them."""
+    L = mb.lib()
+    p = Paged(gpu, mb.BFLOAT16, 16, [4096], [4096], kv_heads=8, dim=64, page=64)
+    q = mb.Tensor.from_bits(gpu, mb.BFLOAT16, bits_of(mb.BFLOAT16, np.random.default_rng(1).standard_normal((4096, 8, 64))))
+    out = mb.Tensor(gpu, mb.BFLOAT16, (4096, 8, 64))
+
+    def ms(limit):
+        mb.check(L.magb200_set_cta_limit(gpu, limit))
+        times = []
+        for _ in range(5):
+            mb.synchronize(gpu)
+            t = time.perf_counter()
+            for _ in range(10):
+                mb.paged_attention(q, p.cache, p.batch, out)
+            mb.synchronize(gpu)
+            times.append(time.perf_counter() - t)
+        return min(times)
+
+    try:
+        assert ms(4) > 5 * ms(0)                                          # 37 times fewer
+    finally:
+        mb.check(L.magb200_set_cta_limit(gpu, 0))
