@@ -905,3 +905,40 @@ def test_the_attention_leaves_multiprocessors_free(gpu):
         assert ms(4) > 5 * ms(0)                                          # 37 times fewer
     finally:
         mb.check(L.magb200_set_cta_limit(gpu, 0))
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("batch", [33, 64, 65, 200])
+@pytest.mark.parametrize("window", [0, 50])
+def test_decode_batches_of_more_sequences_than_lanes(gpu, bits, batch, window):
+    """Single tokens of many sequences, none of some, lengths from none on: the sequences behind the first 32 are counted first and
+    searched afterwards, and pieces end anywhere in the line of all of them."""
+    rng = np.random.default_rng(batch + window)
+    q = [int(n) for n in rng.integers(0, 3, batch)]
+    kv = [int(n) for n in np.exp(rng.uniform(0.0, np.log(700.0), batch))]
+    q[0], q[31], q[32], q[-1], kv[5], kv[40 % batch], kv[-1] = 1, 0, 1, 1, 0, 0, 2000
+    p = Paged(gpu, mb.BFLOAT16, bits, q, kv, kv_heads=3, dim=64, page=16, seed=batch)
+    attend(gpu, p, 6, window=window, pad_rows=1)
+
+
+def test_decode_batch_of_a_thousand_sequences(gpu):
+    p = Paged(gpu, mb.FLOAT16, 16, [1] * 1000, [1 + (i * 37) % 90 for i in range(1000)], kv_heads=1, dim=32, page=16, seed=3)
+    attend(gpu, p, 2)
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("tokens,rows", [(9600, [0, 1, 127, 128, 255, 256, 4863, 9471, 9472, 9599]), (600, [0, 255, 256, 599]), (20, [0, 19])])
+def test_rows_behind_90000_cached_ones(gpu, bits, tokens, rows):
+    """Long walks of the tensor cores' kernel, units whole and in parts, against the definition: the first and last rows of tiles, with
+    the rounding that check_attention counts. Scores spread by 4, so that a row is made of a few of its cached rows, wherever they are."""
+    p = Paged(gpu, mb.BFLOAT16, bits, [tokens], [90000], kv_heads=2, dim=16, page=64, seed=6)
+    qb = bits_of(mb.BFLOAT16, np.random.default_rng(6).standard_normal((tokens, 4, 16)) * 4)
+    got = O.bits_to_f64(mb.BFLOAT16, mb.paged_attention(mb.Tensor.from_bits(gpu, mb.BFLOAT16, qb), p.cache, p.batch).to_bits())
+    q, k, v, u = O.bits_to_f64(mb.BFLOAT16, qb), p.rows("k", 0), p.rows("v", 0), HALF_STEP[mb.BFLOAT16]
+    for r in rows:
+        n = 90000 - tokens + r + 1
+        want, _, spread, size = A.attention(q[r:r + 1], k[:n], v[:n], 0.25, True, 0)
+        weight = 2 * 16 * 2.0 ** -24 * size + 2.0 ** -22 + n * 2.0 ** -24
+        tol = u * np.abs(want) + (u + 2 * weight[..., None]) * spread + 2.0 ** -25
+        assert (tol < np.abs(want).max() / 8).all()                        # what a row of other places would be off by
+        assert (np.abs(got[r:r + 1] - want) <= tol).all(), (r, float((np.abs(got[r:r + 1] - want) / tol).max()))
