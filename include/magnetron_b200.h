@@ -79,7 +79,7 @@ int  magb200_synchronize(int device);
  * on `device`; NULL restores the library's own stream. */
 int  magb200_set_stream(int device, void *cuda_stream);
 void *magb200_get_stream(int device);
-/* Cap the number of CTAs the tensor-core matmuls and the tensor-core attention (sequences of more than 32 (new token, query head)
+/* Cap the number of CTAs the tensor-core matmuls and the tensor-core attention (sequences of more than 16 (new token, query head)
  * rows a KV head) launch on `device` (0 = all 148 SMs; the streaming kernels of decode steps take all). A tensor-parallel caller leaves a
  * few SMs free this way so that a collective running on another stream makes progress beside the persistent GEMM. */
 int  magb200_set_cta_limit(int device, int max_ctas);
@@ -262,7 +262,7 @@ int  magb200_kv_cache_read(int device, const magb200_kv_cache_t *cache, const ma
  * last `window` of them (its own among them). Not causal: all kv_len[b] cached tokens, whatever the number of new ones (cross
  * attention). A row that sees nothing gives 0. lse (optional, f32 [tokens][heads], contiguous): the natural logarithm of the
  * sum of exponentials, -inf for a row that sees nothing. Scores, maxima, sums and the output's sums are fp32; the weights are
- * rounded to the dtype for their product with V (over 8-bit rows to f16 when the sequence has at most 32 (new token, query head)
+ * rounded to the dtype for their product with V (over 8-bit rows to f16 when the sequence has at most 16 (new token, query head)
  * rows a KV head); f16 weights lose bits under 2^-21 of the row's
  * largest, by 2^-32 of it at most. Results are the same from call to call. A cached row that the mask hides
  * from a row does not change it, except that a NaN or infinity in V does within a tile of up to 128 cached rows that the mask

@@ -29,7 +29,7 @@ template <int DT> __device__ __forceinline__ void mma16816(float (&c)[4], const 
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// ---- few rows: stream the cache past 8, 16 or 32 rows -----------------------------------------------------------------------
+// ---- few rows: stream the cache past 8 or 16 rows -----------------------------------------------------------------------------
 // Bound by HBM: a row tile of 8 (token, head) rows needs 16 flop per cached byte. Each warp walks its own tiles of cached rows
 // through a private ring in shared memory (16-byte asynchronous copies), multiplies with mma.sync m16n8k16 and keeps its own
 // maximum, sum and output; the warps meet once at the end. The cached rows are the 16 of the instruction and the queries its
@@ -39,10 +39,10 @@ template <int DT> __device__ __forceinline__ void mma16816(float (&c)[4], const 
 // conversion per two codes); their exponents go to the scores and to the weights, never to the elements.
 constexpr int kFewWarps = 4, kFewThreads = 32 * kFewWarps;
 template <bool kEight, int NT> struct FewCfg {                     // NT: groups of 8 rows
-    static constexpr int kPerSm = NT == 4 ? 1 : NT == 2 && kEight ? 2 : 3;   // CTAs on a multiprocessor
-    static constexpr int kStages = NT == 4 ? 3 : 2;
+    static constexpr int kPerSm = NT == 2 && kEight ? 2 : 3;       // CTAs on a multiprocessor
+    static constexpr int kStages = 2;
     // groups of 16 cached rows in a tile: with codes two groups give a warp twice the independent work between two waits
-    static constexpr int kSubs = kEight && NT < 4 ? 2 : 1;
+    static constexpr int kSubs = kEight ? 2 : 1;
     static constexpr int kTok = 16 * kSubs;
     static constexpr int pitch(int dpad) { return (kEight ? dpad : 2 * dpad) + 16; }   // 16 bytes off a multiple of 128: no bank conflicts
     static constexpr int stage_bytes(int dpad) { return 2 * kTok * pitch(dpad) + (kEight ? 2 * kTok : 0); }
@@ -599,7 +599,7 @@ template <int DT, bool kEight, int DPAD, int NT> int launch_few(const AttentionA
 }
 template <int DT, bool kEight, int DPAD> int launch_few_rows(const AttentionArgs &a, const AttentionPlan &p, cudaStream_t st, bool early) {
     if (p.few_tile == 8) return launch_few<DT, kEight, DPAD, 1>(a, p, st, early);
-    return p.few_tile == 16 ? launch_few<DT, kEight, DPAD, 2>(a, p, st, early) : launch_few<DT, kEight, DPAD, 4>(a, p, st, early);
+    return launch_few<DT, kEight, DPAD, 2>(a, p, st, early);
 }
 template <int DT, bool kEight> int launch_few_dim(const AttentionArgs &a, const AttentionPlan &p, cudaStream_t st, bool early) {
     return a.cache.dim <= 64 ? launch_few_rows<DT, kEight, 64>(a, p, st, early) : launch_few_rows<DT, kEight, 128>(a, p, st, early);
@@ -624,22 +624,27 @@ template <int DT> int launch_all(const AttentionArgs &a, const AttentionPlan &p,
 size_t attention_workspace_bytes() { return (size_t)64 << 20; }
 
 static int few_places(int tile, int bits) {
-    if (tile == 32) return FewCfg<false, 4>::kPerSm;
     return tile == 16 ? (bits == 8 ? FewCfg<true, 2>::kPerSm : FewCfg<false, 2>::kPerSm) : FewCfg<false, 1>::kPerSm;
 }
 
+constexpr int kMostFewRows = 16;
 AttentionPlan plan_attention(const KvCache &c, const KvBatch &b, int heads, bool causal, int64_t window, int sms) {
     AttentionPlan p;
     memset(&p, 0, sizeof(p));
     const int64_t group = heads / c.kv_heads, rows = b.max_q * group;
     int64_t keys = b.max_kv < INT32_MAX ? b.max_kv : INT32_MAX; // cached rows that one row tile sees at most
     if (causal && window > 0 && window + b.max_q + 15 < keys) keys = window + b.max_q + 15;
-    // a warp tile of the streaming form holds 8, 16 or 32 rows; sequences of more rows than that use the tensor cores' tiles. In a
-    // mixed batch the tile is made for the sequences with a single new token.
-    const int64_t fit = rows <= 32 ? rows : group;
-    p.few_tile = fit <= 8 ? 8 : fit <= 16 ? 16 : 32;
+    // A warp tile of the streaming form holds 8 or 16 rows; sequences of more rows than that use the tensor cores' tiles. In a mixed
+    // batch the tile is made for the sequences with a single new token. Measured with 8 KV heads of 128, in us (6 sequences on up to
+    // 50000 rows, 16 and 8 bits; one sequence on 16000 rows of 16 bits):
+    //    8 rows:  in tiles of 8 134, 92 and 27, of 16 136, 121 and 30, on the tensor cores 297, 480 and 35
+    //   16 rows:  in tiles of 16 149, 135 and 42, on the tensor cores 297, 479 and 35
+    //   32 rows:  in tiles of 32, which spilled registers, 363, 431 and 75, on the tensor cores 299, 484 and 35
+    // (64 sequences on up to 4096 rows, 32 rows: 393 and 467 in tiles, 239 and 357 on the tensor cores).
+    const int64_t fit = rows <= kMostFewRows ? rows : group;
+    p.few_tile = fit <= 8 ? 8 : 16;
     p.few_rows = p.few_tile;
-    if (rows <= 32 || (b.batch > 1 && group <= 32)) {
+    if (rows <= kMostFewRows || (b.batch > 1 && group <= kMostFewRows)) {
         // one CTA for every place on the multiprocessors, fewer where there is not enough for pieces of 128 cached rows
         const int64_t pieces = c.kv_heads * ((keys + 127) / 128 + 1), places = (int64_t)few_places(p.few_tile, c.bits) * sms;
         p.few_ctas = (int)(pieces < places && b.batch * pieces < places ? b.batch * pieces : places);
