@@ -39,7 +39,9 @@ template <int DT> __device__ __forceinline__ void mma16816(float (&c)[4], const 
 // conversion per two codes); their exponents go to the scores and to the weights, never to the elements.
 constexpr int kFewWarps = 4, kFewThreads = 32 * kFewWarps;
 template <bool kEight, int NT> struct FewCfg {                     // NT: groups of 8 rows
-    static constexpr int kPerSm = NT == 2 && kEight ? 2 : 3;       // CTAs on a multiprocessor
+    // CTAs on a multiprocessor; us of 64 sequences on up to 4096 rows, 8 KV heads of 128, with two and with three: 16 bits and 8 rows 130
+    // and 136, 16 rows 140 and 149; 8 bits and 8 rows 106 and 89 (four: 124), 16 rows 136 and 182
+    static constexpr int kPerSm = NT == 1 && kEight ? 3 : 2;
     static constexpr int kStages = 2;
     // groups of 16 cached rows in a tile: with codes two groups give a warp twice the independent work between two waits
     static constexpr int kSubs = kEight ? 2 : 1;
@@ -624,7 +626,8 @@ template <int DT> int launch_all(const AttentionArgs &a, const AttentionPlan &p,
 size_t attention_workspace_bytes() { return (size_t)64 << 20; }
 
 static int few_places(int tile, int bits) {
-    return tile == 16 ? (bits == 8 ? FewCfg<true, 2>::kPerSm : FewCfg<false, 2>::kPerSm) : FewCfg<false, 1>::kPerSm;
+    if (tile == 16) return bits == 8 ? FewCfg<true, 2>::kPerSm : FewCfg<false, 2>::kPerSm;
+    return bits == 8 ? FewCfg<true, 1>::kPerSm : FewCfg<false, 1>::kPerSm;
 }
 
 constexpr int kMostFewRows = 16;
