@@ -180,7 +180,7 @@ __device__ __forceinline__ bool find_tile(const AttentionArgs &a, int few_rows, 
 // equally long when a large part has (m n + (m - 1) c) / (1 + k m) of the unit's n blocks; c: what a piece of work costs beside its
 // blocks, in blocks. (64 units of 128 blocks on 148 multiprocessors: 176 us, 261 with every unit in two equal parts; 128
 // units of 133 blocks: 404 us, 411 whole.)
-constexpr int kPieceCost = 3, kLeastBlocks = 4;
+constexpr int kPieceCost = 3, kLeastBlocks = 4, kLongBlocks = 32;
 struct Deal {
     int whole, items;          // units that stay whole; pieces of work of all units
     int cut, k, m, parts;      // units that are cut, into at most `parts` parts
@@ -825,8 +825,15 @@ ManyArgs many_args(const AttentionArgs &a, const AttentionPlan &p) {
     // A unit that is cut has more than 2 kLeastBlocks blocks; fewer than 2 parts for every CTA have to be held. From two rounds on the
     // queue alone keeps the multiprocessors busy, and the second kernel costs what cutting the rest saves (a prefill of 8 x 2048 tokens:
     // 409 us, 417 with its last 136 units in parts).
+    // The bound on the units counts one for every sequence, also those of the streaming kernel. Where it reaches two rounds, but the
+    // rows behind those of single tokens fill less than half a round and a unit may be long, units are cut as well (64 tokens of
+    // 64 heads on 100000 rows beside 60 single tokens, 16 units: 1750 us whole, 370 cut). Short or many units are not worth it (16 single
+    // tokens beside 8 prompts of 500 with a window of 1024, 180 units: 58 us whole, 65 cut; behind 4000 rows: 118 and 128).
     const size_t parts = (size_t)a.ctas * 2 * kManyRows * (a.cache.dim + 4) * sizeof(float);
-    m.split = p.many_tiles * a.cache.kv_heads < 2 * a.ctas && p.many_keys > 2 * kLeastBlocks * kBlock && parts + a.ctas * sizeof(CutUnit) <= a.partial_bytes;
+    const int64_t least_units = (a.batch.tokens * a.group - (int64_t)a.batch.batch * p.few_rows) / kManyRows * a.cache.kv_heads;
+    const bool less_than_two_rounds = p.many_tiles * a.cache.kv_heads < 2 * a.ctas;
+    const bool few_long_units = 2 * least_units < a.ctas && p.many_keys > kLongBlocks * kBlock;
+    m.split = (less_than_two_rounds || few_long_units) && p.many_keys > 2 * kLeastBlocks * kBlock && parts + a.ctas * sizeof(CutUnit) <= a.partial_bytes;
     m.cut_units = reinterpret_cast<CutUnit *>(reinterpret_cast<char *>(a.partial) + parts);
     m.tiles = (int)p.many_tiles;
     m.beside = p.few_ctas > 0;

@@ -942,3 +942,37 @@ def test_rows_behind_90000_cached_ones(gpu, bits, tokens, rows):
         tol = u * np.abs(want) + (u + 2 * weight[..., None]) * spread + 2.0 ** -25
         assert (tol < np.abs(want).max() / 8).all()                        # what a row of other places would be off by
         assert (np.abs(got[r:r + 1] - want) <= tol).all(), (r, float((np.abs(got[r:r + 1] - want) / tol).max()))
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("q_lens,kv_lens,heads,hk,window", [
+    ([64] + [1] * 45, [6000] + [40 + 7 * i for i in range(45)], 32, 8, 0),      # a chunk on a long context beside many single tokens
+    ([1] * 20 + [300, 20, 90] + [1] * 30, [90] * 20 + [2500, 1300, 1700] + [200] * 30, 12, 12, 0),
+    ([1] * 20 + [300, 20, 90] + [1] * 30, [90] * 20 + [2500, 1300, 1700] + [200] * 30, 12, 12, 1100),
+    ([200] * 20 + [1] * 20, [1300] * 40, 8, 8, 0),                              # a round and a rest beside single tokens
+    ([100, 1, 30] + [1] * 120, [9000, 3, 5000] + [50] * 120, 4, 4, 0),          # more single tokens than the chunks' rows
+])
+def test_units_are_cut_beside_single_tokens(gpu, bits, q_lens, kv_lens, heads, hk, window):
+    """Few units of many rows in a batch of many sequences, which the host's bound counts as a unit each."""
+    p = Paged(gpu, mb.BFLOAT16, bits, q_lens, kv_lens, kv_heads=hk, dim=64, page=32, seed=len(q_lens))
+    attend(gpu, p, heads, window=window)
+
+
+def test_a_chunk_takes_no_longer_beside_single_tokens(gpu):
+    """16 units on 100000 cached rows use all multiprocessors, whatever else is in the batch."""
+    def ms(singles):
+        n = 1 + singles
+        p = Paged(gpu, mb.BFLOAT16, 16, [64] + [1] * singles, [100000] + [16] * singles, kv_heads=8, dim=64, page=256)
+        q = mb.Tensor.from_bits(gpu, mb.BFLOAT16, np.zeros((63 + n, 64, 64), np.uint16))
+        out = mb.Tensor(gpu, mb.BFLOAT16, (63 + n, 64, 64))
+        times = []
+        for _ in range(5):
+            mb.synchronize(gpu)
+            t = time.perf_counter()
+            for _ in range(10):
+                mb.paged_attention(q, p.cache, p.batch, out)
+            mb.synchronize(gpu)
+            times.append(time.perf_counter() - t)
+        return min(times)
+
+    assert ms(60) < 3 * ms(0)                                             # 9 times with every unit whole
