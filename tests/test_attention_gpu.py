@@ -976,3 +976,38 @@ def test_a_chunk_takes_no_longer_beside_single_tokens(gpu):
         return min(times)
 
     assert ms(60) < 3 * ms(0)                                             # 9 times with every unit whole
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+def test_caches_beyond_32_bits(gpu, bits):
+    """Pools of more than 2^31 elements (and, with 16 bits, 2^32 bytes); the sequences lie in their first and last pages."""
+    dt, pages, page, hk, dim = mb.BFLOAT16, 17000, 128, 8, 128
+    cache = mb.KVCache(gpu, dt, pages, page, hk, dim, bits)
+    try:
+        tables = [[pages - 1, 0, pages - 3], [pages - 2, pages - 5]]
+        q_lens, kv_lens = [300, 130], [300, 130]
+        rng = np.random.default_rng(bits)
+        kb, vb, qb = (bits_of(dt, rng.standard_normal((430, n, dim))) for n in (hk, hk, 2 * hk))
+        k, v, q = (mb.Tensor.from_bits(gpu, dt, x) for x in (kb, vb, qb))
+        batch = batch_of(gpu, [0, 300, 430], kv_lens, tables)
+        mb.kv_cache_write(cache, batch, k, v)
+        rk, rv = mb.Tensor(gpu, dt, (430, hk, dim)), mb.Tensor(gpu, dt, (430, hk, dim))
+        mb.kv_cache_read(cache, batch, DeviceArray(gpu, np.array([0, 300, 430], np.int32)), rk, rv)
+        back = []
+        for got, raw in ((rk, kb), (rv, vb)):
+            want = raw if bits == 16 else bits_of(dt, A.dequantise(*A.quantise(O.bits_to_f64(dt, raw), dt)))
+            assert np.array_equal(got.to_bits(), want)
+            back.append(O.bits_to_f64(dt, want))
+        many = O.bits_to_f64(dt, mb.paged_attention(q, cache, batch).to_bits())
+        at = np.array([299, 429])                                          # the last new tokens alone: the streaming kernel
+        few = mb.paged_attention(mb.Tensor.from_bits(gpu, dt, qb[at]), cache, batch_of(gpu, [0, 1, 2], kv_lens, tables), None)
+        few = O.bits_to_f64(dt, few.to_bits())
+        for b, rows in enumerate((slice(0, 300), slice(300, 430))):
+            want, _, spread, size = A.attention(O.bits_to_f64(dt, qb[rows]), back[0][rows], back[1][rows], dim ** -0.5, True, 0)
+            weight = 2 * dim * 2.0 ** -24 * size + 2.0 ** -22 + kv_lens[b] * 2.0 ** -24
+            tol = HALF_STEP[dt] * np.abs(want) + (HALF_STEP[dt] + 2 * weight[..., None]) * spread + 2.0 ** -25
+            assert (np.abs(many[rows] - want) <= tol).all() and (np.abs(few[b] - want[-1]) <= tol[-1]).all()
+        mb.synchronize(gpu)
+    finally:
+        del cache
+        mb.check(mb.lib().magb200_pool_trim(gpu))
