@@ -196,7 +196,8 @@ int  magb200_matmul_grouped(int device, const magb200_view_t *x, int count, cons
  * magb200_synchronize / magb200_download as MAGB200_ERR_INVALID_ARG. A sequence with offsets that do not fit is left out; rows in a
  * page outside the cache are not written and not read (the attention takes them for rows of zeros); a length beyond the table
  * is cut to it.
- * None of them allocates after its first call on a device, so all can be recorded into graphs (call the attention once first). */
+ * None of them allocates after its first call on a device, so all can be recorded into graphs (call the attention once first).
+ * Attention calls of a device share its workspace: like the eager ones, graphs that hold them have to run one after the other. */
 
 /* Paged KV cache: `pages` pages of `page_size` tokens (a power of two, 16 or more), one pool for K and one for V, each
  * [pages][kv_heads][page_size][head_dim]; head_dim a multiple of 16, at most 256. bits 16: elements of `dtype` (fp16 / bf16).

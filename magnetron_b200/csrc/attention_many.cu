@@ -19,9 +19,9 @@
 // the rescaling needs no barrier of its own.
 //
 // Work: 4 * 128 * 128 * head_dim flop per tile and block = 1024 clocks of the tensor pipe at head_dim 128, and 16384
-// exponentials = 1024 clocks of the special-function unit. Measured: about 5000 clocks for a block of both tiles, 42 % of either
-// (2368 tokens of 16 heads on 16384 rows, without a mask: 304 us, 900 TFLOP/s; a prefill of 8 x 2048 tokens under the causal mask: 407 us,
-// 675 TFLOP/s). What bounds it is the chain scores -> maximum -> exponentials -> weights -> product of the two tiles, which fall in step,
+// exponentials = 1024 clocks of the special-function unit. Measured: 5200 clocks for a block of both tiles, 39 % of either
+// (2368 tokens of 16 heads on 14016 rows, 110 blocks a multiprocessor, without a mask: 310 us at 1.85 GHz, 880 TFLOP/s; over 8-bit rows 372 us
+// at 1.97 GHz, 6600 clocks; a prefill of 8 x 2048 tokens under the causal mask: 409 us, 672 TFLOP/s). What bounds it is the chain scores -> maximum -> exponentials -> weights -> product of the two tiles, which fall in step,
 // and about 14000 clocks a piece of work beside its blocks. Exponentials by a polynomial on the FMA pipe, a token between the tiles
 // and weights in a place of their own (heads of 64: 255 -> 265 us) cost more than they brought.
 #include "attention_dev.cuh"

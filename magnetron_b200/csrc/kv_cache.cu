@@ -123,8 +123,9 @@ __device__ __forceinline__ void load_runs(const void *base, int64_t row, int u, 
 }
 
 // A CTA takes up to kTurnTokens tokens: their sines are one round of its threads, so that the chain position -> fp64 -> sine ->
-// barrier is paid once for all of them, and their rows follow in one stream. The kernel is bound by its instructions as much as
-// by HBM (a row of 128 is 16 lanes' worth of a hundred of them), so what a lane needs of its place is settled before the loop.
+// barrier is paid once for all of them, and their rows follow in one stream. A row of 128 is 16 lanes' worth of a hundred
+// instructions, so what a lane needs of its place is settled before the loop; even so 53 % of the issue slots are taken, and the 27 warps
+// of a multiprocessor (63 registers a thread) wait for their rows most of the rest (8192 tokens of 72 heads: 68 us, 0.68 of the copy rate).
 constexpr int kTurnTokens = 4;
 template <int DT, int LPR, int kRun, bool kVec>
 __global__ void __launch_bounds__(kRowThreads, 4) qk_norm_rope_kernel(const __grid_constant__ NormRopeArgs a) {
@@ -330,8 +331,8 @@ __global__ void __launch_bounds__(kRowThreads) kv_move_kernel(const __grid_const
     const int u = threadIdx.x % LPR, group = threadIdx.x / LPR;
     const bool mine = 16 * u < c.dim;
     const unsigned rows = 2u * (unsigned)c.kv_heads, total = rows * (unsigned)a.per_cta;
-    // kBatch rows of a group are loaded before the first is used (a write has too much to do per row to gain by it: 45 against
-    // 49 us); all lanes of a warp go round together
+    // kBatch rows of a group are loaded before the first is used; all lanes of a warp go round together. A write has too much to do per
+    // row to gain by it (45 against 49 us): quantising takes 74 % of the issue slots, its integer pipe is busy 69 % of the time.
     constexpr int kBatch = kRead ? 2 : 1;
     for (unsigned base = 0; base < total; base += kBatch * kGroups) {
         int64_t row[kBatch], cell[kBatch];    // element of the packed rows, row of the cache (-1: nothing to do)
