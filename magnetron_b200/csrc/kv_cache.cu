@@ -331,9 +331,11 @@ __global__ void __launch_bounds__(kRowThreads) kv_move_kernel(const __grid_const
     const int u = threadIdx.x % LPR, group = threadIdx.x / LPR;
     const bool mine = 16 * u < c.dim;
     const unsigned rows = 2u * (unsigned)c.kv_heads, total = rows * (unsigned)a.per_cta;
-    // kBatch rows of a group are loaded before the first is used; all lanes of a warp go round together. A write has too much to do per
-    // row to gain by it (45 against 49 us): quantising takes 74 % of the issue slots, its integer pipe is busy 69 % of the time.
-    constexpr int kBatch = kRead ? 2 : 1;
+    // kBatch rows of a group are loaded before the first is used; all lanes of a warp go round together. Of 16 bits two rows are
+    // worth it (us with one and with two: write of 32768 tokens 48.7 and 45.8, read of long sequences 122.1 and 119.2); with codes there is
+    // too much to do per row (write 42.7 and 49, read 99.9 and 101.4): quantising takes 74 % of the issue slots, the integer pipe is busy
+    // 69 % of the time.
+    constexpr int kBatch = kEight ? 1 : 2;
     for (unsigned base = 0; base < total; base += kBatch * kGroups) {
         int64_t row[kBatch], cell[kBatch];    // element of the packed rows, row of the cache (-1: nothing to do)
         bool is_v[kBatch];
