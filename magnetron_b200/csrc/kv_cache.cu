@@ -265,14 +265,11 @@ constexpr int kMaxTokensPerCta = 16;
 struct Slot { int64_t page; int offset; };   // page < 0: nothing to do for this token
 
 // The page and slot of position `pos` of sequence b. Bounds are checked here: what does not fit raises the word and is skipped.
-__device__ __forceinline__ Slot locate(const KvCache &c, const KvBatch &b, int seq, int64_t kv, int64_t pos) {
+__device__ __forceinline__ Slot locate(const KvCache &c, const KvBatch &b, int seq, int64_t pos) {
     Slot s;
     s.page = -1;
     s.offset = (int)(pos & (c.page_size - 1));
-    if (pos < 0) {                            // fewer cached tokens than new ones: this one has no place
-        if (kv < 0) atomicOr(b.status + kBatchWord, kBadLength);
-        return s;
-    }
+    if (pos < 0) return s;                    // fewer cached tokens than new ones: this one has no place
     const int64_t entry = pos >> c.page_shift;
     if (entry >= b.max_pages) { atomicOr(b.status + kBatchWord, kBadLength); return s; }
     const int32_t page = b.table[(int64_t)seq * b.max_pages + entry];
@@ -317,11 +314,13 @@ __global__ void __launch_bounds__(kRowThreads) kv_move_kernel(const __grid_const
         if (t < a.batch.tokens) {
             const int seq = find_sequence(a.cu, a.batch.batch, t, lane);
             const int64_t begin = a.cu[seq], end = a.cu[seq + 1], kv = a.batch.kv_len[seq];
-            if (t >= begin && t < end && offsets_fit<kRead>(a.batch, begin, end)) {      // rows behind the last sequence belong to nobody
+            // rows behind the last sequence belong to nobody; those of one whose offsets do not fit (offsets_fit) are not moved
+            if (t >= begin && t < end && begin >= 0 && end <= a.batch.tokens && (kRead || end - begin <= a.batch.max_q)) {
                 const int64_t pos = kRead ? t - begin : kv - (end - t);
                 if (lane == 0) {
                     if (kRead && pos >= kv) atomicOr(a.batch.status + kBatchWord, kBadLength);   // more rows asked for than are cached
-                    else s = locate(c, a.batch, seq, kv, pos);
+                    else if (!kRead && kv < 0) atomicOr(a.batch.status + kBatchWord, kBadLength);
+                    else s = locate(c, a.batch, seq, pos);
                 }
             }
         }
@@ -331,11 +330,11 @@ __global__ void __launch_bounds__(kRowThreads) kv_move_kernel(const __grid_const
     const int u = threadIdx.x % LPR, group = threadIdx.x / LPR;
     const bool mine = 16 * u < c.dim;
     const unsigned rows = 2u * (unsigned)c.kv_heads, total = rows * (unsigned)a.per_cta;
-    // kBatch rows of a group are loaded before the first is used; all lanes of a warp go round together. Of 16 bits two rows are
-    // worth it (us with one and with two: write of 32768 tokens 48.7 and 45.8, read of long sequences 122.1 and 119.2); with codes there is
-    // too much to do per row (write 42.7 and 49, read 99.9 and 101.4): quantising takes 74 % of the issue slots, the integer pipe is busy
-    // 69 % of the time.
-    constexpr int kBatch = kEight ? 1 : 2;
+    // kBatch rows of a group are loaded before the first is used; all lanes of a warp go round together (us with one and
+    // with two: 16-bit write of 32768 tokens 48.7 and 45.8, 16-bit read of long sequences 122.1 and 119.2, 8-bit read 99.0 and 97.7). A
+    // write to 8 bits has too much to do per row (42.7 and 49): quantising takes 74 % of the issue slots, the integer pipe is busy 69 % of
+    // the time.
+    constexpr int kBatch = !kEight || kRead ? 2 : 1;
     for (unsigned base = 0; base < total; base += kBatch * kGroups) {
         int64_t row[kBatch], cell[kBatch];    // element of the packed rows, row of the cache (-1: nothing to do)
         bool is_v[kBatch];
