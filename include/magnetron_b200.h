@@ -215,8 +215,8 @@ typedef struct magb200_kv_cache_t {
 /* The sequences of a call. New tokens are packed: sequence b owns rows cu_q[b] .. cu_q[b + 1] - 1 of q, k, v and out (cu_q[0]
  * = 0, ascending, equal for a sequence without new tokens; rows from cu_q[batch] on belong to nobody and are left alone).
  * kv_len[b] counts its cached tokens INCLUDING its new ones, which are its last cu_q[b + 1] - cu_q[b]; a new token whose position
- * would be negative has no place. A negative kv_len is an error if the sequence has new tokens, and counts as 0. pages[b][i] is the page of positions i * page_size and up; sequences may share pages that
- * the call does not write. max_q and max_kv bound the new and cached tokens of any sequence (0: all rows / the whole table):
+ * would be negative has no place. A negative kv_len is an error if the sequence has new tokens, and counts as 0. pages[b][i] is the
+ * page of positions i * page_size and up; sequences may share pages that the call does not write. max_q and max_kv bound the new and cached tokens of any sequence (0: all rows / the whole table):
  * a sequence with more new tokens than max_q is an error, max_kv only steers how work is split. Device pointers. A sequence whose
  * own offsets do not fit is skipped as a whole; rows that offsets which do not ascend give to several sequences come from any of them. */
 typedef struct magb200_kv_batch_t {
@@ -264,9 +264,8 @@ int  magb200_kv_cache_read(int device, const magb200_kv_cache_t *cache, const ma
  * attention). A row that sees nothing gives 0. lse (optional, f32 [tokens][heads], contiguous): the natural logarithm of the
  * sum of exponentials, -inf for a row that sees nothing. Scores, maxima, sums and the output's sums are fp32; the weights are
  * rounded to the dtype for their product with V (over 8-bit rows to f16 when the sequence has at most 16 (new token, query head)
- * rows a KV head); f16 weights lose bits under 2^-21 of the row's
- * largest, by 2^-32 of it at most. Results are the same from call to call. A cached row that the mask hides
- * from a row does not change it, except that a NaN or infinity in V does within a tile of up to 128 cached rows that the mask
+ * rows a KV head); f16 weights lose bits under 2^-21 of the row's largest, by 2^-32 of it at most. Results are the same from call
+ * to call. A cached row that the mask hides from a row does not change it, except that a NaN or infinity in V does within a tile of up to 128 cached rows that the mask
  * crosses; rows of a page behind the last cached token are never used. */
 int  magb200_paged_attention(int device, const magb200_view_t *q, const magb200_kv_cache_t *cache, const magb200_kv_batch_t *batch,
                              double scale, int causal, int64_t window, const magb200_view_t *out, const magb200_view_t *lse);
